@@ -23,6 +23,12 @@ sliding layers, and transformers' attention-function interface:
     FlashSWDAWithLearnedSinks.apply(q, k, v, sinks, window_size, sink_size=0, softmax_scale=None)
     register_transformers("fa_gfx950")   # attn_implementation="fa_gfx950"
 
+Answering with a model (paged.py): a paged key-value cache, one new token a sequence, eviction:
+    paged_append(k, v, k_pages, v_pages, block_table, lens, cu_seqlens=None, descale=(1.0, 1.0))
+    paged_attention(q, k_pages, v_pages, block_table, lens, window_size=None, sink_size=0, sinks=None,
+                    scale=None, descale=(1.0, 1.0), max_seqlen=None, weight_sums=None)
+    paged_evict(k_pages, v_pages, block_table, lens, weight_sums, keep, new_table, sink_size=0, recent=0)
+
 The directory name is not a Python identifier; import it with
 ``importlib.import_module("flashattention-gpt-oss-finetuning_amd")`` from the repository root.
 """
@@ -30,6 +36,7 @@ from .attention import (FlashSWDAWithLearnedSinks, FlashSWDAWithSink, FlashSWDAW
                         FlashSWDAWithSinkVarlen, flash_swda_with_sink, flash_swda_with_sink_fp8,
                         flash_swda_with_sink_varlen, quantize_fp8, swa_sink_attention, swa_sink_attention_split)
 from .gpt_oss import attention, gpt_oss_attention_forward, padded_attention, register_transformers  # noqa: F401
+from .paged import paged_append, paged_attention, paged_evict  # noqa: F401
 from .flops import Workload, allowed_pairs_per_head  # noqa: F401
 
 __all__ = [
@@ -47,6 +54,9 @@ __all__ = [
     "gpt_oss_attention_forward",
     "padded_attention",
     "register_transformers",
+    "paged_append",
+    "paged_attention",
+    "paged_evict",
     "Workload",
     "allowed_pairs_per_head",
 ]

@@ -32,6 +32,7 @@ FA_ERR_LAUNCH = -8
 FA_ERR_OVERFLOW = -9
 FA_ERR_SCALE = -10
 FA_ERR_SCRATCH = -11
+FA_ERR_PAGES = -12
 FA_SCRATCH_BYTES = 72 << 20
 
 # Every function the header declares; the tests check that the library exports each one.
@@ -51,6 +52,11 @@ EXPORTS = (
     "fa_fwd_fp8_pv",
     "fa_quantize_fp8",
     "fa_quantize_fp8_amax",
+    "fa_paged_append",
+    "fa_paged_workspace_bytes",
+    "fa_paged_attention",
+    "fa_paged_evict_workspace_bytes",
+    "fa_paged_evict",
     "fa_bwd_workspace_bytes",
     "fa_bwd_full_workspace_bytes",
     "fa_check_fwd",
@@ -118,6 +124,68 @@ class BwdParams(ctypes.Structure):
     ]
 
 
+_i64x2 = ctypes.c_int64 * 2
+
+
+class PagedCache(ctypes.Structure):
+    _fields_ = [
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("k_stride", _i64x3),
+        ("v_stride", _i64x3),
+        ("table", ctypes.c_void_p),
+        ("lens", ctypes.c_void_p),
+        ("table_stride", ctypes.c_int64),
+        ("batch", ctypes.c_int32),
+        ("pages", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("table_width", ctypes.c_int32),
+        ("heads_kv", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("k_descale", ctypes.c_double),
+        ("v_descale", ctypes.c_double),
+    ]
+
+
+class PagedAttentionParams(ctypes.Structure):
+    _fields_ = [
+        ("cache", PagedCache),
+        ("q", ctypes.c_void_p),
+        ("o", ctypes.c_void_p),
+        ("q_stride", _i64x2),
+        ("o_stride", _i64x2),
+        ("sinks", ctypes.c_void_p),
+        ("weight_sums", ctypes.c_void_p),
+        ("sums_stride", _i64x2),
+        ("sums_width", ctypes.c_int32),
+        ("heads_q", ctypes.c_int32),
+        ("max_len", ctypes.c_int32),
+        ("window", ctypes.c_int32),
+        ("sink", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("softmax_scale", ctypes.c_float),
+    ]
+
+
+class PagedEvictParams(ctypes.Structure):
+    _fields_ = [
+        ("cache", PagedCache),
+        ("sums", ctypes.c_void_p),
+        ("new_sums", ctypes.c_void_p),
+        ("sums_stride", _i64x2),
+        ("new_sums_stride", _i64x2),
+        ("new_table", ctypes.c_void_p),
+        ("new_table_stride", ctypes.c_int64),
+        ("new_lens", ctypes.c_void_p),
+        ("sums_width", ctypes.c_int32),
+        ("new_table_width", ctypes.c_int32),
+        ("keep", ctypes.c_int32),
+        ("sink", ctypes.c_int32),
+        ("recent", ctypes.c_int32),
+    ]
+
+
 _lock = threading.Lock()
 _lib = None
 
@@ -168,6 +236,16 @@ def lib() -> ctypes.CDLL:
             L.fa_quantize_fp8_amax.argtypes = [ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64] + [ctypes.c_void_p] * 5
             L.fa_bwd_full_workspace_bytes.argtypes = [ctypes.c_int32] * 9
             L.fa_bwd_full_workspace_bytes.restype = ctypes.c_size_t
+            L.fa_paged_append.argtypes = [ctypes.POINTER(PagedCache), ctypes.c_void_p, ctypes.c_void_p,
+                                          ctypes.POINTER(ctypes.c_int64), ctypes.POINTER(ctypes.c_int64), ctypes.c_int32,
+                                          ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p]
+            L.fa_paged_workspace_bytes.argtypes = [ctypes.POINTER(PagedAttentionParams)]
+            L.fa_paged_workspace_bytes.restype = ctypes.c_size_t
+            L.fa_paged_attention.argtypes = [ctypes.POINTER(PagedAttentionParams), ctypes.c_void_p, ctypes.c_size_t,
+                                             ctypes.c_void_p]
+            L.fa_paged_evict_workspace_bytes.argtypes = [ctypes.c_int32] * 3
+            L.fa_paged_evict_workspace_bytes.restype = ctypes.c_size_t
+            L.fa_paged_evict.argtypes = [ctypes.POINTER(PagedEvictParams), ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
             L.fa_check_fwd.argtypes = [ctypes.POINTER(FwdParams)]
             L.fa_check_fwd.restype = ctypes.c_int
             L.fa_check_bwd.argtypes = [ctypes.POINTER(BwdParams)]

@@ -461,3 +461,198 @@ def backward_varlen(q, k, v, o, lse, do, cu_seqlens, max_seqlen: int, window: in
     if sinks is None:
         return dq, dk, dv
     return dq, dk, dv, dsinks
+
+
+# ---- paged key-value caches -------------------------------------------------------------------
+
+_PAGE_DTYPES = {**_DTYPES, torch.float8_e4m3fn: _lib.FA_DTYPE_FP8_E4M3}
+
+
+def _on_device(t, first, name, first_name):
+    if t.device != first.device:
+        raise RuntimeError(f"{name} is on {t.device} but {first_name} is on {first.device}")
+
+
+def _fits_i32(x: int, name: str) -> int:
+    if not _I32_MIN <= x <= _I32_MAX:
+        raise ValueError(f"{name} does not fit 32 bits")
+    return x
+
+
+def _refuse_traced(what: str) -> None:
+    if torch.jit.is_tracing() or torch.compiler.is_compiling():
+        raise RuntimeError(f"{what} works on tensors in place: it cannot be traced or transformed")
+
+
+def _paged_cache(k_pages, v_pages, block_table, lens, k_descale, v_descale):
+    """(the cache's parameter block, what it points to)."""
+    if k_pages.device.type != "cuda":
+        raise RuntimeError(f"k_pages is on {k_pages.device}: the gfx950 attention kernels need GPU tensors "
+                           "(there is no CPU implementation)")
+    for t, n in ((v_pages, "v_pages"), (block_table, "block_table"), (lens, "lens")):
+        _on_device(t, k_pages, n, "k_pages")
+    if k_pages.dim() != 4 or v_pages.shape != k_pages.shape:
+        raise ValueError("k_pages and v_pages must both be [pages, Hkv, page_size, D], got "
+                         f"{list(k_pages.shape)} and {list(v_pages.shape)}")
+    if v_pages.dtype != k_pages.dtype:
+        raise ValueError("v_pages has a different dtype than k_pages")
+    if k_pages.dtype not in _PAGE_DTYPES:
+        raise ValueError(f"k_pages has dtype {k_pages.dtype}; supported dtypes are bfloat16, float16, float32 and float8_e4m3fn")
+    if k_pages.dtype != torch.float8_e4m3fn and (k_descale != 1.0 or v_descale != 1.0):
+        raise ValueError("descale is for float8_e4m3fn pages only")
+    if k_pages.numel() == 0:
+        raise ValueError(f"k_pages must not be empty, got {list(k_pages.shape)}")
+    for t in (k_pages, v_pages):
+        m = 16 // t.element_size() - 1
+        st = t.stride()
+        if st[3] != 1 or (st[0] & m) or (st[1] & m) or (st[2] & m) or (t.data_ptr() & 15):
+            raise ValueError("pages are used in place: their head-dim stride must be 1, the other strides multiples of 16 "
+                             "bytes and their base 16-byte aligned")
+    if block_table.dim() != 2 or block_table.dtype != torch.int32 or block_table.shape[0] < 1 or block_table.shape[1] < 1:
+        raise ValueError(f"block_table must be int32 [B, width], got {list(block_table.shape)}")
+    if lens.dim() != 1 or lens.dtype != torch.int32 or lens.shape[0] != block_table.shape[0]:
+        raise ValueError(f"lens must be int32 [B] with the block_table's B, got {list(lens.shape)}")
+    table = _table_ready(block_table)
+    lens = lens.contiguous()
+    c = _lib.PagedCache()
+    c.k, c.v, c.table, c.lens = k_pages.data_ptr(), v_pages.data_ptr(), table.data_ptr(), lens.data_ptr()
+    c.k_stride[:], c.v_stride[:] = _strides3(k_pages), _strides3(v_pages)
+    c.table_stride = table.stride(0)
+    c.batch, c.table_width = (_fits_i32(n, "the block_table's shape") for n in table.shape)
+    c.pages, c.heads_kv, c.page_size, c.head_dim = (_fits_i32(n, "the pages' shape") for n in k_pages.shape)
+    c.dtype = _PAGE_DTYPES[k_pages.dtype]
+    c.k_descale, c.v_descale = k_descale, v_descale
+    return c, (table, lens)
+
+
+def _table_ready(t):
+    return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
+
+
+def _paged_input(t, k_pages, name):
+    """A [rows, H, D] input: of the pages' type (16 bits over e4m3 pages), copied where the kernels cannot read it."""
+    _on_device(t, k_pages, name, "k_pages")
+    if t.dim() != 3 or t.shape[2] != k_pages.shape[3]:
+        raise ValueError(f"{name} must be 3-D with the pages' head dim {k_pages.shape[3]}, got {list(t.shape)}")
+    e4m3 = k_pages.dtype == torch.float8_e4m3fn
+    if t.dtype not in (torch.bfloat16, torch.float16) if e4m3 else t.dtype != k_pages.dtype:
+        raise ValueError(f"{name} has dtype {t.dtype} over pages of {k_pages.dtype}; both must have the same type, or bfloat16 "
+                         "or float16 over float8_e4m3fn pages")
+    m = 16 // t.element_size() - 1
+    if t.stride(2) != 1 or (t.stride(0) & m) or (t.stride(1) & m) or (t.data_ptr() & 15):
+        return t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def _check_sums(sums, k_pages, B):
+    _on_device(sums, k_pages, "weight_sums", "k_pages")
+    if (sums.dtype != torch.float32 or sums.dim() != 3 or sums.shape[0] != B or sums.shape[1] != k_pages.shape[1]
+            or (sums.stride(2) != 1 and sums.shape[2] != 1)):
+        raise ValueError("weight_sums must be float32 [B, Hkv, tokens], next to each other in the last dimension, got "
+                         f"{list(sums.shape)}")
+
+
+def _changed(*tensors):
+    """What a call wrote in place, as far as autograd's version counters go."""
+    for t in tensors:
+        if not t.is_inference():
+            torch.autograd.graph.increment_version(t)
+
+
+def _run_paged(fn, device, *args):
+    with _DeviceGuard(device):
+        stream = ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+        rc = getattr(_lib.lib(), fn)(*args, stream)
+    _lib.raise_for_status(rc, fn)
+
+
+def paged_append(k, v, k_pages, v_pages, block_table, lens, cu, k_descale: float, v_descale: float) -> None:
+    """fa_paged_append; cu: int32 offsets [B + 1] on the device, or None."""
+    b = _binding()
+    if b is not None:
+        return b.paged_append(k, v, k_pages, v_pages, block_table, lens, cu, k_descale, v_descale)
+    _refuse_traced("paged_append")
+    c, held = _paged_cache(k_pages, v_pages, block_table, lens, k_descale, v_descale)
+    k, v = _paged_input(k, k_pages, "k"), _paged_input(v, k_pages, "v")
+    if k.shape[1] != k_pages.shape[1] or v.shape != k.shape or v.dtype != k.dtype:
+        raise ValueError(f"k and v must both be [rows, Hkv, D] of one dtype, got {list(k.shape)} and {list(v.shape)}")
+    if cu is not None and (cu.device != k.device or cu.dtype != torch.int32 or cu.dim() != 1 or not cu.is_contiguous()
+                           or cu.shape[0] != c.batch + 1):
+        raise ValueError(f"cu_seqlens must hold B + 1 offsets, got {list(cu.shape)}")
+    if cu is None and k.shape[0] != c.batch:
+        raise ValueError(f"without cu_seqlens k and v have one row a sequence, got {list(k.shape)}")
+    strides = [(ctypes.c_int64 * 2)(t.stride(1), t.stride(0)) for t in (k, v)]
+    _run_paged("fa_paged_append", k.device, ctypes.byref(c), ctypes.c_void_p(k.data_ptr()), ctypes.c_void_p(v.data_ptr()), *strides,
+               _fits_i32(k.shape[0], "the number of rows"), _DTYPES[k.dtype], ctypes.c_void_p(None if cu is None else cu.data_ptr()))
+    _changed(k_pages, v_pages)
+
+
+def paged_attention(q, k_pages, v_pages, block_table, lens, window: int, sink: int, sinks, scale: float, k_descale: float,
+                    v_descale: float, max_len: int, weight_sums):
+    """fa_paged_attention: o [B, Hq, D]."""
+    b = _binding()
+    if b is not None:
+        return b.paged_attention(q, k_pages, v_pages, block_table, lens, window, sink, sinks, scale, k_descale, v_descale, max_len,
+                                 weight_sums)
+    _refuse_traced("paged_attention")
+    p = _lib.PagedAttentionParams()
+    p.cache, held = _paged_cache(k_pages, v_pages, block_table, lens, k_descale, v_descale)
+    q = _paged_input(q, k_pages, "q")
+    B, Hq, D = q.shape
+    if B != block_table.shape[0] or Hq < 1 or Hq % k_pages.shape[1]:
+        raise ValueError("q must be [B, Hq, D] with the block_table's B and a multiple of the pages' heads, got "
+                         f"{list(q.shape)}")
+    sk = None if sinks is None else _sinks_ready(sinks, Hq, q.device)
+    o = torch.empty((B, Hq, D), dtype=q.dtype, device=q.device)
+    p.q, p.o = q.data_ptr(), o.data_ptr()
+    p.q_stride[:], p.o_stride[:] = q.stride()[:2], o.stride()[:2]
+    p.sinks = None if sk is None else sk.data_ptr()
+    if weight_sums is not None:
+        _check_sums(weight_sums, k_pages, B)
+        p.weight_sums = weight_sums.data_ptr()
+        p.sums_stride[:] = weight_sums.stride()[:2]
+        p.sums_width = _i32(weight_sums.shape[2])
+    p.heads_q, p.max_len = _fits_i32(Hq, "the number of heads"), _i32(max_len)
+    p.window, p.sink = _i32(window), _i32(sink)
+    p.dtype = _DTYPES[q.dtype]
+    p.softmax_scale = scale
+    with _DeviceGuard(q.device):  # (the size depends on the device's number of compute units)
+        nbytes = int(_lib.lib().fa_paged_workspace_bytes(ctypes.byref(p)))
+    ws = torch.empty((max(nbytes, 256),), dtype=torch.uint8, device=q.device)
+    _run_paged("fa_paged_attention", q.device, ctypes.byref(p), ctypes.c_void_p(ws.data_ptr()), ctypes.c_size_t(ws.numel()))
+    if weight_sums is not None:
+        _changed(weight_sums)
+    return o
+
+
+def paged_evict(k_pages, v_pages, block_table, lens, weight_sums, keep: int, new_table, sink: int, recent: int):
+    """fa_paged_evict: (new lens, new weight sums)."""
+    b = _binding()
+    if b is not None:
+        return tuple(b.paged_evict(k_pages, v_pages, block_table, lens, weight_sums, keep, new_table, sink, recent))
+    _refuse_traced("paged_evict")
+    p = _lib.PagedEvictParams()
+    p.cache, held = _paged_cache(k_pages, v_pages, block_table, lens, 1.0, 1.0)
+    B, Hkv = p.cache.batch, p.cache.heads_kv
+    _on_device(weight_sums, k_pages, "weight_sums", "k_pages")
+    _on_device(new_table, k_pages, "new_table", "k_pages")
+    _check_sums(weight_sums, k_pages, B)
+    if new_table.dim() != 2 or new_table.dtype != torch.int32 or new_table.shape[0] != B or new_table.shape[1] < 1:
+        raise ValueError(f"new_table must be int32 [B, width], got {list(new_table.shape)}")
+    if new_table.data_ptr() == block_table.data_ptr():
+        raise ValueError("new_table must name other pages than block_table")
+    new_table = _table_ready(new_table)
+    new_lens = torch.empty((B,), dtype=torch.int32, device=lens.device)
+    new_sums = torch.empty(weight_sums.shape, dtype=torch.float32, device=lens.device)
+    p.sums, p.new_sums = weight_sums.data_ptr(), new_sums.data_ptr()
+    p.sums_stride[:], p.new_sums_stride[:] = weight_sums.stride()[:2], new_sums.stride()[:2]
+    p.sums_width = _i32(weight_sums.shape[2])
+    p.new_table, p.new_table_stride = new_table.data_ptr(), new_table.stride(0)
+    p.new_table_width = _fits_i32(new_table.shape[1], "the new_table's width")
+    p.new_lens = new_lens.data_ptr()
+    p.keep, p.sink, p.recent = _fits_i32(keep, "keep"), _fits_i32(sink, "sink_size"), _fits_i32(recent, "recent")
+    nbytes = int(_lib.lib().fa_paged_evict_workspace_bytes(B, Hkv, p.keep))
+    ws = torch.empty((max(nbytes, 256),), dtype=torch.uint8, device=lens.device)
+    _run_paged("fa_paged_evict", lens.device, ctypes.byref(p), ctypes.c_void_p(ws.data_ptr()), ctypes.c_size_t(ws.numel()))
+    _changed(k_pages, v_pages)
+    return new_lens, new_sums

@@ -889,6 +889,7 @@ const char* fa_strerror(int status) {
     case FA_ERR_OVERFLOW: return "problem size exceeds the kernels' index range";
     case FA_ERR_SCALE: return "softmax_scale (and the fp8 dequantisation factors) must be finite";
     case FA_ERR_SCRATCH: return "the problem needs more backward workspace than the library's scratch buffer (FA_SCRATCH_BYTES) holds; use fa_bwd with a workspace";
+    case FA_ERR_PAGES: return "invalid paged cache: pages, page size, table width and keep must be >= 1, sink and recent >= 0 and together at most keep, weight sums as wide as the table's tokens and the new table as wide as keep";
   }
   return "unknown fa_status";
 }

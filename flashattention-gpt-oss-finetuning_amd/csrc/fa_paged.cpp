@@ -1,0 +1,250 @@
+// fa_paged.cpp - the C ABI of the paged key-value cache (include/fa_gfx950.h): host-side validation, workspace sizing and
+// launch shapes.  Nothing is launched and no HIP call made before the arguments have been checked.
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+
+#include "../../include/fa_gfx950.h"
+#include "fa_args.h"
+#include "fa_paged.h"
+
+namespace {
+
+bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+bool strides_ok(const int64_t* s, int n, int elem_bytes) {
+  for (int i = 0; i < n; ++i)
+    if (s[i] < 0 || (s[i] & (16 / elem_bytes - 1)) != 0) return false;
+  return true;
+}
+int elem_bytes(int32_t dtype) { return dtype == FA_DTYPE_F32 ? 4 : dtype == FA_DTYPE_FP8_E4M3 ? 1 : 2; }
+size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
+
+int check_cache(const fa_paged_cache& c) {
+  if (!c.k || !c.v || !c.table || !c.lens) return FA_ERR_NULL;
+  if (c.batch < 1 || c.heads_kv < 1) return FA_ERR_SHAPE;
+  if (c.pages < 1 || c.page_size < 1 || c.table_width < 1) return FA_ERR_PAGES;
+  const int D = c.head_dim;
+  if (D != 16 && D != 32 && D != 64 && D != 128) return FA_ERR_HEAD_DIM;
+  if (c.dtype < FA_DTYPE_BF16 || c.dtype > FA_DTYPE_F32) return FA_ERR_DTYPE;
+  const int eb = elem_bytes(c.dtype);
+  if (eb == 1 && D < 64) return FA_ERR_HEAD_DIM;
+  if (!aligned(c.k, 16) || !aligned(c.v, 16) || !aligned(c.table, 4) || !aligned(c.lens, 4) || c.table_stride < 0 ||
+      !strides_ok(c.k_stride, 3, eb) || !strides_ok(c.v_stride, 3, eb))
+    return FA_ERR_ALIGN;
+  if (int64_t(c.table_width) * c.page_size >= fa::kPagedMaxTokens) return FA_ERR_OVERFLOW;
+  return FA_OK;
+}
+
+// a call's element type against its cache's
+bool types_ok(int32_t dtype, int32_t cache) {
+  if (dtype != FA_DTYPE_BF16 && dtype != FA_DTYPE_F16 && dtype != FA_DTYPE_F32) return false;
+  return cache == dtype || (cache == FA_DTYPE_FP8_E4M3 && dtype != FA_DTYPE_F32);
+}
+
+fa::PagedCache cache_args(const fa_paged_cache& c) {
+  fa::PagedCache r{};
+  const int eb = elem_bytes(c.dtype);
+  r.k = static_cast<uint8_t*>(c.k);
+  r.v = static_cast<uint8_t*>(c.v);
+  for (int i = 0; i < 3; ++i) {
+    r.sk[i] = c.k_stride[i] * eb;
+    r.sv[i] = c.v_stride[i] * eb;
+  }
+  r.table = c.table;
+  r.lens = c.lens;
+  r.table_stride = c.table_stride;
+  r.B = c.batch;
+  r.pages = c.pages;
+  r.page_size = c.page_size;
+  r.table_width = c.table_width;
+  r.Hkv = c.heads_kv;
+  r.max_len = c.table_width * c.page_size;
+  r.div = fa::page_div(uint32_t(c.page_size));
+  return r;
+}
+
+int status(hipError_t e) { return e == hipSuccess ? FA_OK : FA_ERR_LAUNCH; }
+
+// Sequences of at most this many visible keys are taken whole, a workgroup each, in one launch.
+constexpr int kWholeKeys = 512;
+// Workgroups of a split call's launch for each compute unit, and the fewest units worth a workgroup of their own.
+constexpr int kPartsPerCu = 2, kLeastUnits = 2;
+
+struct Plan {
+  int max_units, row_tiles, parts;
+  size_t part_o, part_ml, lse, logits;  // bytes
+  size_t bytes() const { return std::max<size_t>(256, part_o + part_ml + lse + logits); }
+};
+
+int plan(const fa_paged_attention_params* p, Plan* r) {
+  if (!p) return FA_ERR_NULL;
+  const fa_paged_cache& c = p->cache;
+  const int rc = check_cache(c);
+  if (rc != FA_OK) return rc;
+  if (!p->q || !p->o) return FA_ERR_NULL;
+  if (p->heads_q < 1 || p->heads_q % c.heads_kv != 0 || p->max_len < 1) return FA_ERR_SHAPE;
+  if (!types_ok(p->dtype, c.dtype)) return FA_ERR_DTYPE;
+  if (p->window < 1 && p->sink < 1) return FA_ERR_MASK;
+  const bool q8 = c.dtype == FA_DTYPE_FP8_E4M3;
+  if (!std::isfinite(p->softmax_scale) || (q8 && (!std::isfinite(float(p->softmax_scale * c.k_descale)) || !std::isfinite(float(c.v_descale)))))
+    return FA_ERR_SCALE;
+  const int eb = elem_bytes(p->dtype);
+  if (!aligned(p->q, 16) || !aligned(p->o, 16) || !strides_ok(p->q_stride, 2, eb) || !strides_ok(p->o_stride, 2, eb) ||
+      !aligned(p->sinks, 4) || !aligned(p->weight_sums, 4))
+    return FA_ERR_ALIGN;
+  const int max_len = int(std::min<int64_t>(int64_t(c.table_width) * c.page_size, p->max_len));
+  if (p->weight_sums) {
+    if (p->sums_stride[0] < 0 || p->sums_stride[1] < 0) return FA_ERR_ALIGN;
+    if (p->sums_width < max_len) return FA_ERR_PAGES;
+  }
+  const int64_t most = std::min<int64_t>(max_len, int64_t(std::max(p->window, 0)) + std::max(p->sink, 0));
+  const int G = p->heads_q / c.heads_kv;
+  r->max_units = fa::paged_units(int(most));
+  r->row_tiles = (G + 15) / 16;
+  const int64_t streams = int64_t(c.heads_kv) * r->row_tiles, units = int64_t(c.batch) * r->max_units;
+  if (units >= (int64_t(1) << 31) || !fa::grid_fits(std::max(streams, int64_t(p->heads_q)) * c.batch)) return FA_ERR_OVERFLOW;
+  r->parts = 0;
+  if (most > kWholeKeys) {
+    const int64_t want = std::max<int64_t>(1, int64_t(kPartsPerCu) * fa::device_cus() / streams);
+    r->parts = int(std::min(want, (units + kLeastUnits - 1) / kLeastUnits));
+    if (!fa::grid_fits(streams * r->parts)) return FA_ERR_OVERFLOW;
+  }
+  const size_t slots = size_t(streams) * r->parts * 2;
+  r->part_o = align256(slots * 16 * c.head_dim * sizeof(float));
+  r->part_ml = align256(slots * 32 * sizeof(float));
+  r->lse = r->logits = 0;
+  if (p->weight_sums) {
+    r->lse = align256(size_t(c.batch) * p->heads_q * sizeof(float));
+    r->logits = align256(size_t(units) * p->heads_q * fa::kPagedUnit * sizeof(float));
+    // (the launch that adds up the weights: a workgroup for 1024 keys, at least one a (sequence, KV head))
+    if (!fa::grid_fits((r->max_units + 7) / 8 * int64_t(c.heads_kv) * c.batch)) return FA_ERR_OVERFLOW;
+  }
+  return FA_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int fa_paged_append(const fa_paged_cache* c, const void* k, const void* v, const int64_t k_stride[2],
+                    const int64_t v_stride[2], int32_t rows, int32_t dtype, const int32_t* cu_seqlens, void* stream) {
+  if (!c || !k_stride || !v_stride) return FA_ERR_NULL;
+  const int rc = check_cache(*c);
+  if (rc != FA_OK) return rc;
+  if (rows < 0 || (!cu_seqlens && rows != c->batch)) return FA_ERR_SHAPE;
+  if (!types_ok(dtype, c->dtype)) return FA_ERR_DTYPE;
+  const int eb = elem_bytes(dtype);
+  if (!aligned(k, 16) || !aligned(v, 16) || !aligned(cu_seqlens, 4) || !strides_ok(k_stride, 2, eb) || !strides_ok(v_stride, 2, eb))
+    return FA_ERR_ALIGN;
+  fa::AppendArgs a{};
+  if (c->dtype == FA_DTYPE_FP8_E4M3) {
+    a.k_inv = float(1.0 / c->k_descale);
+    a.v_inv = float(1.0 / c->v_descale);
+    if (!std::isfinite(c->k_descale) || !std::isfinite(c->v_descale) || !std::isfinite(a.k_inv) || !std::isfinite(a.v_inv))
+      return FA_ERR_SCALE;
+  }
+  if (rows == 0) return FA_OK;
+  if (!k || !v) return FA_ERR_NULL;
+  a.c = cache_args(*c);
+  a.k = static_cast<const uint8_t*>(k);
+  a.v = static_cast<const uint8_t*>(v);
+  for (int i = 0; i < 2; ++i) {
+    a.sk[i] = k_stride[i] * eb;
+    a.sv[i] = v_stride[i] * eb;
+  }
+  a.cu = cu_seqlens;
+  a.rows = rows;
+  if (!fa::grid_fits((int64_t(rows) + 3) / 4)) return FA_ERR_OVERFLOW;
+  return status(fa::launch_paged_append(a, dtype, c->dtype, c->head_dim, static_cast<hipStream_t>(stream)));
+}
+
+size_t fa_paged_workspace_bytes(const fa_paged_attention_params* p) {
+  Plan r;
+  return plan(p, &r) == FA_OK ? r.bytes() : 0;
+}
+
+int fa_paged_attention(const fa_paged_attention_params* p, void* workspace, size_t workspace_bytes, void* stream) {
+  Plan r;
+  const int rc = plan(p, &r);
+  if (rc != FA_OK) return rc;
+  if (!workspace || !aligned(workspace, 256) || workspace_bytes < r.bytes()) return FA_ERR_WORKSPACE;
+  const fa_paged_cache& c = p->cache;
+  const bool q8 = c.dtype == FA_DTYPE_FP8_E4M3;
+  fa::PagedAttnArgs a{};
+  a.c = cache_args(c);
+  a.c.max_len = std::min(a.c.max_len, p->max_len);
+  a.q = static_cast<const uint8_t*>(p->q);
+  a.o = static_cast<uint8_t*>(p->o);
+  const int eb = elem_bytes(p->dtype);
+  for (int i = 0; i < 2; ++i) {
+    a.sq[i] = p->q_stride[i] * eb;
+    a.so[i] = p->o_stride[i] * eb;
+    a.ssum[i] = p->sums_stride[i];
+  }
+  a.sinks = p->sinks;
+  a.sums = p->weight_sums;
+  a.Hq = p->heads_q;
+  a.G = p->heads_q / c.heads_kv;
+  a.row_tiles = r.row_tiles;
+  a.W = std::min(std::max(p->window, 0), a.c.max_len);
+  a.S = std::min(std::max(p->sink, 0), a.c.max_len);
+  a.c2 = float(double(p->softmax_scale) * 1.4426950408889634 * (q8 ? c.k_descale : 1.0));
+  a.oscale = q8 ? float(c.v_descale) : 1.f;
+  a.max_units = r.max_units;
+  a.parts = r.parts;
+  a.least = kLeastUnits;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  a.part_o = reinterpret_cast<float*>(ws);
+  a.part_ml = reinterpret_cast<float*>(ws + r.part_o);
+  a.lse = reinterpret_cast<float*>(ws + r.part_o + r.part_ml);
+  a.logits = reinterpret_cast<float*>(ws + r.part_o + r.part_ml + r.lse);
+  return status(fa::launch_paged_attention(a, p->dtype, c.dtype, c.head_dim, static_cast<hipStream_t>(stream)));
+}
+
+size_t fa_paged_evict_workspace_bytes(int32_t batch, int32_t heads_kv, int32_t keep) {
+  if (batch < 1 || heads_kv < 1 || keep < 1) return 0;
+  return align256(size_t(batch) * heads_kv * keep * sizeof(int32_t));
+}
+
+int fa_paged_evict(const fa_paged_evict_params* p, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!p) return FA_ERR_NULL;
+  const fa_paged_cache& c = p->cache;
+  const int rc = check_cache(c);
+  if (rc != FA_OK) return rc;
+  if (!p->sums || !p->new_sums || !p->new_table || !p->new_lens) return FA_ERR_NULL;
+  const int64_t tokens = int64_t(c.table_width) * c.page_size;
+  if (p->keep < 1 || p->sink < 0 || p->recent < 0 || int64_t(p->sink) + p->recent > p->keep || p->sums_width < tokens ||
+      p->new_table_width < 1 || int64_t(p->new_table_width) * c.page_size < p->keep)
+    return FA_ERR_PAGES;
+  if (p->keep >= fa::kPagedMaxTokens) return FA_ERR_OVERFLOW;
+  if (!aligned(p->sums, 4) || !aligned(p->new_sums, 4) || !aligned(p->new_table, 4) || !aligned(p->new_lens, 4) ||
+      p->new_table_stride < 0)
+    return FA_ERR_ALIGN;
+  for (int i = 0; i < 2; ++i)
+    if (p->sums_stride[i] < 0 || p->new_sums_stride[i] < 0) return FA_ERR_ALIGN;
+  if (!workspace || !aligned(workspace, 256) || workspace_bytes < fa_paged_evict_workspace_bytes(c.batch, c.heads_kv, p->keep))
+    return FA_ERR_WORKSPACE;
+  const int row = c.head_dim * elem_bytes(c.dtype);
+  // workgroups of the two launches: 1024 threads a (sequence, KV head), and 1024 pieces of 16 bytes of kept entries
+  const int64_t heads = int64_t(c.batch) * c.heads_kv, chunk = 1024 / (row / 16);
+  if (!fa::grid_fits(heads, 1024) || !fa::grid_fits(heads * ((p->keep + chunk - 1) / chunk))) return FA_ERR_OVERFLOW;
+  fa::EvictArgs a{};
+  a.c = cache_args(c);
+  a.sums = p->sums;
+  a.new_sums = p->new_sums;
+  for (int i = 0; i < 2; ++i) {
+    a.ssum[i] = p->sums_stride[i];
+    a.snew[i] = p->new_sums_stride[i];
+  }
+  a.sums_width = p->sums_width;
+  a.new_table = p->new_table;
+  a.new_table_stride = p->new_table_stride;
+  a.new_lens = p->new_lens;
+  a.keep = p->keep;
+  a.S = p->sink;
+  a.R = p->recent;
+  a.kept = static_cast<int*>(workspace);
+  return status(fa::launch_paged_evict(a, row, static_cast<hipStream_t>(stream)));
+}
+
+}  // extern "C"

@@ -1,0 +1,75 @@
+// fa_paged.h - kernel argument blocks of the paged key-value cache, shared by the C ABI (fa_paged.cpp) and the kernels.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "fa_paged_plan.h"
+
+namespace fa {
+
+// The cache as the kernels read it.  Strides are in bytes; offsets are formed in 64 bits.
+struct PagedCache {
+  uint8_t* k;
+  uint8_t* v;
+  int64_t sk[3], sv[3];   // page, head, slot
+  const int* table;       // [B][table_width], rows table_stride entries apart
+  const int* lens;
+  int64_t table_stride;
+  int B, pages, page_size, table_width, Hkv;
+  int max_len;            // lens are cut off here; at most table_width * page_size
+  PageDiv div;
+};
+
+struct AppendArgs {
+  PagedCache c;
+  const uint8_t* k;
+  const uint8_t* v;
+  int64_t sk[2], sv[2];   // head, row
+  const int* cu;          // NULL: row b belongs to sequence b
+  int rows;
+  float k_inv, v_inv;     // e4m3 pages: reciprocals of the descales
+};
+
+struct PagedAttnArgs {
+  PagedCache c;
+  const uint8_t* q;
+  uint8_t* o;
+  int64_t sq[2], so[2];   // batch, head
+  const float* sinks;     // NULL, or [Hq] learned logits
+  float* sums;            // NULL, or accumulated weights [B][Hkv][max_len]
+  int64_t ssum[2];
+  int Hq, G, row_tiles;   // heads a group, tiles of 16 heads in it
+  int W, S;
+  float c2;               // softmax scale * log2(e) * K's descale: scores are exp2(c2 * q.k)
+  float oscale;           // V's descale
+  int max_units;          // units of a sequence of max_len tokens
+  // split calls: the runs a (KV head, row tile) is cut into, 0 where every workgroup takes a whole sequence
+  int parts, least;
+  // workspace
+  float* part_o;          // [Hkv row_tiles][parts][2][16][D]
+  float* part_ml;         // [Hkv row_tiles][parts][2][2][16]: maximum (log2 domain), sum
+  float* lse;             // with sums: [B][Hq] (log2 domain)
+  float* logits;          // with sums: [Hkv][B][max_units][G][kPagedUnit] (log2 domain)
+};
+
+struct EvictArgs {
+  PagedCache c;
+  const float* sums;
+  float* new_sums;
+  int64_t ssum[2], snew[2];
+  int sums_width;
+  const int* new_table;
+  int64_t new_table_stride;
+  int* new_lens;
+  int keep, S, R;
+  int* kept;              // workspace: [B][Hkv][keep] entries kept, in order
+};
+
+// dtype and cache are fa_dtype values
+hipError_t launch_paged_append(const AppendArgs& a, int dtype, int cache, int D, hipStream_t s);
+hipError_t launch_paged_attention(const PagedAttnArgs& a, int dtype, int cache, int D, hipStream_t s);
+// row_bytes: of a head's entry
+hipError_t launch_paged_evict(const EvictArgs& a, int row_bytes, hipStream_t s);
+
+}  // namespace fa

@@ -1,0 +1,591 @@
+// fa_paged_attn.hip - attention of one new token a sequence over a paged key-value cache (fa_paged_attention).
+//
+// For each (sequence, KV head) the G query heads of its group meet the n visible keys:
+//     s[h, k] = scale q[h] . K[k],   lse[h] = log(sum_k exp s[h, k] + exp(sink[h])),   o[h] = sum_k exp(s[h, k] - lse[h]) V[k].
+// 4 G operations a cache element, so the cache's bytes bound it: the kernel is built to keep them coming.
+//
+// paged_attn_kernel.  A workgroup of 4 waves takes a run of keys for 16 query heads (a group, padded); its waves
+// take tiles of 32 keys in turn and meet only at the run's end.  A tile goes from memory to registers to the
+// matrix instructions, without LDS and without a lane seeing another's values:
+//   * S^T = K Q^T as v_mfma_f32_16x16x32 with the keys as rows.  Lane l (r = l % 16, j = l / 16) supplies key rows r of two
+//     16-key halves and gets, for head r, rows 4j..4j+3 of both.  Half T's row 4j + i is the tile's key 8j + 4T + i, so the
+//     lane's eight scores are those of keys 8j..8j+7.
+//   * O^T = V^T P^T with the head dim as rows: the lane's eight weights are the B operand as they lie, and the A
+//     operand is eight V entries of keys 8j..8j+7, of which the lane loads D / 16 neighbouring dims each and pairs
+//     two keys' halves (one v_perm per register).  Its C rows are the lane's own head again, so
+//     maximum, sum and rescaling need no exchange.
+// The running maximum is raised only where a score exceeds it by more than 2^8 (weights stay within float32 and
+// 16 bits), which after the first tiles hardly ever happens; only then do lanes exchange maxima.
+// P goes into the 16-bit product as the sum of two 16-bit parts (P rounded, and what that left), so o carries its own
+// rounding only; the second product costs matrix time that the loads leave idle.  float32 uses v_mfma_f32_16x16x4.
+//
+// Keys are addressed through an LDS table of 64-bit offsets, filled for 512 keys at a time: key -> page -> offset is
+// worked out once a key.  A key on no page (an entry outside [0, pages)) and the keys past the end have offset -1; their
+// scores become -inf and their V entries 0, whatever lies in memory.
+//
+// Runs.  With a workgroup a (KV head, sequence) long sequences would leave the chip idle, and with a fixed number of
+// pieces a sequence ragged batches would.  Split calls deal out the units of all sequences evenly
+// (fa_paged_plan.h): each workgroup finds its run by a prefix sum over lens, on the device, so the grid depends on
+// sizes the host knows.  Pieces that are no whole sequence leave (maximum, sum, o) in the workspace, and
+// paged_join_kernel adds them in order.
+#include <hip/hip_runtime.h>
+
+#include "../../include/fa_gfx950.h"
+#include "fa_common.h"
+#include "fa_paged.h"
+
+namespace fa {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWaves = 4;
+constexpr int kTile = 32;
+constexpr int kFill = 512;  // keys of an LDS offset table
+
+__device__ __forceinline__ int seq_len(const PagedCache& c, int b) { return imin(imax(c.lens[b], 0), c.max_len); }
+
+__device__ __forceinline__ int wave_prefix(int n, int lane) {  // inclusive
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int y = __shfl_up(n, o);
+    if (lane >= o) n += y;
+  }
+  return n;
+}
+
+__device__ __forceinline__ int units_of(const PagedAttnArgs& a, int b) {
+  return b < a.c.B ? paged_units(visible(seq_len(a.c, b), a.W, a.S).count) : 0;
+}
+
+// Units of the sequences before b, and of all of them (every lane of the wave calls).
+__device__ __forceinline__ void units_before(const PagedAttnArgs& a, int b, int& before, int& total) {
+  const int lane = threadIdx.x & 63;
+  before = total = 0;
+  for (int b0 = 0; b0 < a.c.B; b0 += 64) {
+    const int n = units_of(a, b0 + lane);
+    const int x = wave_prefix(n, lane);
+    if (b >= b0 && b < b0 + 64) before = total + __builtin_amdgcn_readfirstlane(__shfl(x - n, b - b0));
+    total += __builtin_amdgcn_readfirstlane(__shfl(x, 63));
+  }
+}
+
+// The sequence that holds unit u < total, and its first unit.
+__device__ __forceinline__ void find_unit(const PagedAttnArgs& a, int u, int& b, int& start) {
+  const int lane = threadIdx.x & 63;
+  int base = 0;
+  for (int b0 = 0; b0 < a.c.B; b0 += 64) {
+    const int n = units_of(a, b0 + lane);
+    const int x = wave_prefix(n, lane);
+    const unsigned long long m = __ballot(base + x > u);
+    if (m) {
+      const int l = __builtin_amdgcn_readfirstlane(__ffsll(m) - 1);
+      b = b0 + l;
+      start = base + __builtin_amdgcn_readfirstlane(__shfl(x - n, l));
+      return;
+    }
+    base += __builtin_amdgcn_readfirstlane(__shfl(x, 63));
+  }
+  b = 0;  // (not reached: u < total)
+  start = 0;
+}
+
+// Element types.  EB, CB: bytes of a query and of a cache element.
+struct PBF16 : BF16 {
+  static constexpr int EB = 2, CB = 2;
+};
+struct PF16 : F16 {
+  static constexpr int EB = 2, CB = 2;
+};
+struct PBF16Q8 : BF16 {
+  static constexpr int EB = 2, CB = 1;
+  static __device__ __forceinline__ uint32_t widen(uint32_t x, bool hi) {
+    return hi ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, 1.0f, true))
+              : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, 1.0f, false));
+  }
+};
+struct PF16Q8 : F16 {
+  static constexpr int EB = 2, CB = 1;
+  static __device__ __forceinline__ uint32_t widen(uint32_t x, bool hi) {
+    return hi ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, 1.0f, true))
+              : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, 1.0f, false));
+  }
+};
+struct PF32 {
+  static constexpr int EB = 4, CB = 4;
+};
+
+__device__ __forceinline__ float quarters_max(float x) {
+  x = fmaxf(x, __shfl_xor(x, 16));
+  return fmaxf(x, __shfl_xor(x, 32));
+}
+__device__ __forceinline__ float quarters_sum(float x) {
+  x += __shfl_xor(x, 16);
+  return x + __shfl_xor(x, 32);
+}
+
+// One wave's tile of 32 keys in registers.
+template <typename E, int D>
+struct Tile {
+  static constexpr int ROW = D * E::CB;                      // bytes of an entry
+  static constexpr int NK = ROW >= 64 ? ROW / 64 : 1;        // 16-byte pieces of an entry that a lane holds
+  static constexpr int VB = ROW / 16;                        // bytes of a V entry that a lane holds
+  static constexpr int VD = VB >= 4 ? VB / 4 : 1;
+  u32x4 k[2][NK];
+  uint32_t v[8][VD];
+  bool gone;  // some key of the tile is on no page or past the end
+};
+
+template <typename E, int D>
+struct Wave {
+  using T = Tile<E, D>;
+  static constexpr int NC = D / 16;                          // dims a lane of the output holds of each 16 rows
+  static constexpr bool F = E::EB == 4;
+  static constexpr int NQ = F ? D / 16 : (D >= 32 ? D / 32 : 1);
+  u32x4 q[NQ];
+  f32x4 acc[NC];
+  float m, mref, l;  // running maximum (log2 domain), the same with 0 for none, this lane's sum
+
+  // Q as the B operand: head r of the tile, dims in the order in which the K pieces hold them.
+  __device__ __forceinline__ void load_q(const uint8_t* q_row, bool have) {
+    const int j = (threadIdx.x & 63) >> 4;
+#pragma unroll
+    for (int f = 0; f < NQ; ++f) {
+      // 16-byte piece 4f + j of the row; an e4m3 piece holds 16 dims, two pieces of q
+      const int piece = E::CB == 1 ? 2 * (4 * (f / 2) + j) + f % 2 : 4 * f + j;
+      q[f] = have && piece * 16 < D * E::EB ? ld16(q_row + 16 * piece) : zero16();
+    }
+  }
+  __device__ __forceinline__ void reset() {
+#pragma unroll
+    for (int c = 0; c < NC; ++c) acc[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+    m = kNegInf;
+    mref = 0.f;
+    l = 0.f;
+  }
+
+  // off: the tile's 32 offsets of K, and of V, in LDS.
+  static __device__ __forceinline__ void load(T& t, const uint8_t* k, const uint8_t* v, const int64_t* koff, const int64_t* voff) {
+    const int lane = threadIdx.x & 63, r = lane & 15, j = lane >> 4;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int64_t o = koff[8 * (r >> 2) + 4 * h + (r & 3)];
+      const uint8_t* p = k + (o < 0 ? 0 : o);
+#pragma unroll
+      for (int n = 0; n < T::NK; ++n) t.k[h][n] = 64 * n + 16 * j < T::ROW ? ld16(p + 64 * n + 16 * j) : zero16();
+    }
+    bool gone = false;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int64_t o = voff[8 * j + e];
+      gone |= o < 0;
+      const uint8_t* p = v + (o < 0 ? 0 : o) + T::VB * r;
+      if constexpr (T::VB == 2) {
+        t.v[e][0] = *reinterpret_cast<const uint16_t*>(p);
+      } else if constexpr (T::VB == 4) {
+        t.v[e][0] = *reinterpret_cast<const uint32_t*>(p);
+      } else if constexpr (T::VB == 8) {
+        const u32x2 x = *reinterpret_cast<const u32x2*>(p);
+        t.v[e][0] = x[0];
+        t.v[e][1] = x[1];
+      } else {
+#pragma unroll
+        for (int w = 0; w < T::VB / 16; ++w) {
+          const u32x4 x = ld16(p + 16 * w);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) t.v[e][4 * w + i] = x[i];
+        }
+      }
+    }
+    t.gone = wave_any(gone);
+  }
+
+  // Eight keys' values of dim c of this lane as an A operand: v[e] holds D / 16 dims of key 8j + e.
+  static __device__ __forceinline__ u32x4 v_frag(const uint32_t (&v)[8][NC >= 2 ? NC / 2 : 1], int c) {
+    u32x4 f;
+#pragma unroll
+    for (int d = 0; d < 4; ++d)
+      f[d] = __builtin_amdgcn_perm(v[2 * d + 1][c / 2], v[2 * d][c / 2], c % 2 ? 0x07060302u : 0x05040100u);
+    return f;
+  }
+
+  // voff: the tile's offsets (for tiles with keys that do not count); logits: where the lane's eight scores go, or NULL
+  __device__ __forceinline__ void step(T& t, float c2, const int64_t* voff, float* logits) {
+    const int lane = threadIdx.x & 63, j = lane >> 4;
+    f32x4 s0 = {0.f, 0.f, 0.f, 0.f}, s1 = s0;
+    if constexpr (F) {
+#pragma unroll
+      for (int n = 0; n < T::NK; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t k0 = t.k[0][n][e], k1 = t.k[1][n][e], qe = q[n][e];
+          s0 = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, k0), __builtin_bit_cast(float, qe), s0, 0, 0, 0);
+          s1 = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, k1), __builtin_bit_cast(float, qe), s1, 0, 0, 0);
+        }
+    } else {
+#pragma unroll
+      for (int n = 0; n < T::NK; ++n) {
+        if constexpr (E::CB == 1) {
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            u32x4 k0, k1;
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+              k0[2 * w] = E::widen(t.k[0][n][2 * u + w], false);
+              k0[2 * w + 1] = E::widen(t.k[0][n][2 * u + w], true);
+              k1[2 * w] = E::widen(t.k[1][n][2 * u + w], false);
+              k1[2 * w + 1] = E::widen(t.k[1][n][2 * u + w], true);
+            }
+            s0 = E::mfma16(k0, q[2 * n + u], s0);
+            s1 = E::mfma16(k1, q[2 * n + u], s1);
+          }
+        } else {
+          s0 = E::mfma16(t.k[0][n], q[n], s0);
+          s1 = E::mfma16(t.k[1][n], q[n], s1);
+        }
+      }
+    }
+    float s[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      s[i] = s0[i] * c2;
+      s[4 + i] = s1[i] * c2;
+    }
+    if (t.gone) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const bool ok = voff[8 * j + e] >= 0;
+        s[e] = ok ? s[e] : kNegInf;
+#pragma unroll
+        for (int w = 0; w < T::VD; ++w) t.v[e][w] = ok ? t.v[e][w] : 0u;
+      }
+    }
+    if (logits) {
+      *reinterpret_cast<f32x4*>(logits) = f32x4{s[0], s[1], s[2], s[3]};
+      *reinterpret_cast<f32x4*>(logits + 4) = f32x4{s[4], s[5], s[6], s[7]};
+    }
+    float mx = s[0];
+#pragma unroll
+    for (int e = 1; e < 8; ++e) mx = fmaxf(mx, s[e]);
+    if (wave_any(mx > m + 8.f)) {
+      const float up = fmaxf(m, quarters_max(mx));
+      const float scale = m == kNegInf ? 0.f : fast_exp2(m - up);
+      l *= scale;
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[c][i] *= scale;
+      m = up;
+      mref = m == kNegInf ? 0.f : m;
+    }
+    float p[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      p[e] = fast_exp2(s[e] - mref);
+      l += p[e];
+    }
+    if constexpr (F) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+          acc[c] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, t.v[e][c]), p[e], acc[c], 0, 0, 0);
+    } else {
+      const u32x4 hi = pack8<E>(p);
+      float rest[8];
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        rest[2 * w] = p[2 * w] - E::to_f32(uint16_t(hi[w]));
+        rest[2 * w + 1] = p[2 * w + 1] - E::to_f32(uint16_t(hi[w] >> 16));
+      }
+      const u32x4 lo = pack8<E>(rest);
+      if constexpr (E::CB == 1) {
+        uint32_t w[8][NC / 2];
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+#pragma unroll
+          for (int d = 0; d < NC / 2; ++d) w[e][d] = E::widen(t.v[e][d / 2], d % 2);
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          const u32x4 f = v_frag(w, c);
+          acc[c] = E::mfma16(f, hi, acc[c]);
+          acc[c] = E::mfma16(f, lo, acc[c]);
+        }
+      } else {
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          const u32x4 f = v_frag(t.v, c);
+          acc[c] = E::mfma16(f, hi, acc[c]);
+          acc[c] = E::mfma16(f, lo, acc[c]);
+        }
+      }
+    }
+  }
+};
+
+// D / 16 output values of one head (float32) to o, in its type.
+template <typename E, int N>
+__device__ __forceinline__ void store_out(uint8_t* o, const float (&x)[N]) {
+  if constexpr (E::EB == 4) {
+    if constexpr (N == 1) *reinterpret_cast<float*>(o) = x[0];
+    else if constexpr (N == 2) *reinterpret_cast<f32x2*>(o) = f32x2{x[0], x[1]};
+    else {
+#pragma unroll
+      for (int i = 0; i < N; i += 4) *reinterpret_cast<f32x4*>(o + 4 * i) = f32x4{x[i], x[i + 1], x[i + 2], x[i + 3]};
+    }
+  } else if constexpr (N == 1) {
+    *reinterpret_cast<uint16_t*>(o) = uint16_t(E::pack2(x[0], x[0]));
+  } else {
+    uint32_t w[N / 2];
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) w[i] = E::pack2(x[2 * i], x[2 * i + 1]);
+    if constexpr (N == 2) *reinterpret_cast<uint32_t*>(o) = w[0];
+    else if constexpr (N == 4) *reinterpret_cast<u32x2*>(o) = u32x2{w[0], w[1]};
+    else st16(o, u32x4{w[0], w[1], w[2], w[3]});
+  }
+}
+
+template <int D>
+struct Shared {
+  static constexpr int PAD = D + 4;  // float32 rows 4 banks apart
+  union {
+    struct {
+      int64_t k[kFill], v[kFill];
+    } off;
+    float o[kWaves][16][PAD];
+  };
+  float m[kWaves][16], l[kWaves][16];
+};
+
+template <typename E, int D>
+__global__ __launch_bounds__(kThreads) void paged_attn_kernel(const PagedAttnArgs a) {
+  constexpr int NC = D / 16;
+  __shared__ Shared<D> sh;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r = lane & 15, j = lane >> 4;
+  const int streams = a.c.Hkv * a.row_tiles;
+  const int stream = blockIdx.x % streams, part = blockIdx.x / streams;
+  const int hkv = stream / a.row_tiles, h0 = stream % a.row_tiles * 16;  // first head of the tile within the group
+  const int heads = imin(16, a.G - h0);
+  const uint8_t* kb = a.c.k + int64_t(hkv) * a.c.sk[1];
+  const uint8_t* vb = a.c.v + int64_t(hkv) * a.c.sv[1];
+
+  int b, start, u, end;  // the run's sequence, its first unit, the run's units [u, end)
+  int per = 0;
+  if (a.parts == 0) {
+    b = part;
+    start = u = 0;
+    end = 1;
+  } else {
+    int none, total;
+    units_before(a, 0, none, total);
+    per = units_per_part(total, a.parts, a.least);
+    if (int64_t(part) * per >= total) return;
+    u = part * per;
+    end = imin(total, u + per);
+    find_unit(a, u, b, start);
+  }
+
+  Wave<E, D> w;
+  // (b < B, v0 >= 0 and the join's last part hold by themselves, unless lens change under a running call: then the results
+  // mean nothing, but no access leaves the tensors)
+  while (u < end && b < a.c.B) {
+    const Visible vis = visible(seq_len(a.c, b), a.W, a.S);
+    const int units = paged_units(vis.count);
+    if (a.parts == 0) end = units;
+    const int stop = imin(end, start + units);
+    const bool whole = u == start && stop == start + units;
+    const int v0 = imax(0, (u - start) * kPagedUnit), v1 = imin(vis.count, (stop - start) * kPagedUnit);
+    const int head = hkv * a.G + h0 + r;
+    w.load_q(a.q + int64_t(b) * a.sq[0] + int64_t(r < heads ? head : hkv * a.G) * a.sq[1], r < heads);
+    w.reset();
+    const int* table = a.c.table + int64_t(b) * a.c.table_stride;
+    for (int f0 = v0; f0 < v1; f0 += kFill) {
+      const int fill = imin(kFill, v1 - f0), tiles = (fill + kTile - 1) / kTile;
+      for (int i = tid; i < tiles * kTile; i += kThreads) {
+        int64_t ko = -1, vo = -1;
+        if (i < fill) {
+          const int key = visible_key(vis, f0 + i), pi = page_of(a.c.div, key);
+          const int page = table[pi], slot = key - pi * a.c.page_size;
+          if (page >= 0 && page < a.c.pages) {
+            ko = int64_t(page) * a.c.sk[0] + int64_t(slot) * a.c.sk[2];
+            vo = int64_t(page) * a.c.sv[0] + int64_t(slot) * a.c.sv[2];
+          }
+        }
+        sh.off.k[i] = ko;
+        sh.off.v[i] = vo;
+      }
+      __syncthreads();
+      Tile<E, D> t;
+      if (wave < tiles) w.load(t, kb, vb, sh.off.k + kTile * wave, sh.off.v + kTile * wave);
+      for (int i = wave; i < tiles; i += kWaves) {
+        Tile<E, D> next;
+        const int n = i + kWaves;
+        if (n < tiles) w.load(next, kb, vb, sh.off.k + kTile * n, sh.off.v + kTile * n);
+        float* logits = nullptr;
+        if (a.sums && r < heads) {
+          const int at = f0 + kTile * i;
+          logits = a.logits + (((int64_t(hkv) * a.c.B + b) * a.max_units + at / kPagedUnit) * a.G + h0 + r) * kPagedUnit +
+                   at % kPagedUnit + 8 * j;
+        }
+        w.step(t, a.c2, sh.off.v + kTile * i, logits);
+        if (n < tiles) t = next;
+      }
+      __syncthreads();
+    }
+
+    // the four waves' results, in wave order
+    const float l = quarters_sum(w.l);
+    if (j == 0) {
+      sh.m[wave][r] = w.m;
+      sh.l[wave][r] = l;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int c = 0; c < NC; ++c) sh.o[wave][r][(4 * j + i) * NC + c] = w.acc[c][i];
+    __syncthreads();
+    const int oh = tid >> 4, od = (tid & 15) * NC;  // this thread's head and dims
+    float m = kNegInf;
+#pragma unroll
+    for (int x = 0; x < kWaves; ++x) m = fmaxf(m, sh.m[x][oh]);
+    const float ref = m == kNegInf ? 0.f : m;
+    float sum = 0.f, o[NC] = {};
+#pragma unroll
+    for (int x = 0; x < kWaves; ++x) {
+      const float f = fast_exp2(sh.m[x][oh] - ref);
+      sum += f * sh.l[x][oh];
+#pragma unroll
+      for (int c = 0; c < NC; ++c) o[c] += f * sh.o[x][oh][od + c];
+    }
+    if (oh < heads) {
+      const int hq = hkv * a.G + h0 + oh;
+      if (whole) {
+        float ls = sum, scale = 1.f;
+        if (a.sinks) {
+          const float sink = a.sinks[hq] * kLog2e, top = fmaxf(m, sink);
+          if (top != kNegInf) {
+            scale = fast_exp2(ref - top);
+            ls = (m == kNegInf ? 0.f : sum * scale) + fast_exp2(sink - top);
+            m = top;
+          }
+        }
+        const float inv = ls == 0.f || sum == 0.f ? 0.f : scale * a.oscale / ls;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) o[c] = sum == 0.f ? 0.f : o[c] * inv;
+        store_out<E, NC>(a.o + int64_t(b) * a.so[0] + int64_t(hq) * a.so[1] + od * E::EB, o);
+        if (a.sums && (tid & 15) == 0) a.lse[int64_t(b) * a.Hq + hq] = (m == kNegInf ? 0.f : m) + fast_log2(ls);
+      } else {
+        const int64_t slot = int64_t(stream) * a.parts * 2 + part_slot(part, per, start);
+        float* po = a.part_o + (slot * 16 + oh) * D + od;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) po[c] = o[c];
+        if ((tid & 15) == 0) {
+          a.part_ml[slot * 32 + oh] = m;
+          a.part_ml[slot * 32 + 16 + oh] = sum;
+        }
+      }
+    }
+    __syncthreads();
+    u = stop;
+    start += units;
+    ++b;
+  }
+}
+
+// A query head of a sequence that was cut: its pieces' results, added in order.  64 threads.
+template <typename E, int D>
+__global__ __launch_bounds__(64) void paged_join_kernel(const PagedAttnArgs a) {
+  const int hq = blockIdx.x % a.Hq, b = blockIdx.x / a.Hq;
+  int start, total;
+  units_before(a, b, start, total);
+  const int per = units_per_part(total, a.parts, a.least);
+  const int units = units_of(a, b), first = start / per, last = imin(a.parts - 1, (start + units - 1) / per);
+  if (first >= last) return;
+  const int hkv = hq / a.G, h = hq % a.G, stream = hkv * a.row_tiles + h / 16, oh = h % 16;
+  const int64_t base = int64_t(stream) * a.parts * 2;
+  const int lane = threadIdx.x;
+  float m = kNegInf;
+  for (int p = first + lane; p <= last; p += 64) m = fmaxf(m, a.part_ml[(base + part_slot(p, per, start)) * 32 + oh]);
+#pragma unroll
+  for (int x = 32; x >= 1; x >>= 1) m = fmaxf(m, __shfl_xor(m, x));
+  float top = m;
+  const float sink = a.sinks ? a.sinks[hq] * kLog2e : kNegInf;
+  top = fmaxf(top, sink);
+  const float ref = top == kNegInf ? 0.f : top;
+  constexpr int ND = (D + 63) / 64;
+  float sum = 0.f, o[ND] = {};
+  for (int p = first; p <= last; ++p) {
+    const int64_t slot = base + part_slot(p, per, start);
+    const float f = fast_exp2(a.part_ml[slot * 32 + oh] - ref);
+    sum += f * a.part_ml[slot * 32 + 16 + oh];
+    if (f != 0.f) {
+#pragma unroll
+      for (int i = 0; i < ND; ++i)
+        if (lane + 64 * i < D) o[i] += f * a.part_o[(slot * 16 + oh) * D + lane + 64 * i];
+    }
+  }
+  const float ls = sum + (sink == kNegInf ? 0.f : fast_exp2(sink - ref));
+  const float inv = sum == 0.f ? 0.f : a.oscale / ls;
+  uint8_t* out = a.o + int64_t(b) * a.so[0] + int64_t(hq) * a.so[1];
+#pragma unroll
+  for (int i = 0; i < ND; ++i)
+    if (lane + 64 * i < D) {
+      const float x[1] = {sum == 0.f ? 0.f : o[i] * inv};
+      store_out<E, 1>(out + (lane + 64 * i) * E::EB, x);
+    }
+  if (a.sums && lane == 0) a.lse[int64_t(b) * a.Hq + hq] = ref + fast_log2(ls);
+}
+
+// sums[b, hkv, key] += sum over the group's heads of 2^(logit - lse), a thread a key: no order to choose, no atomics.
+constexpr int kSumKeys = 1024;
+__global__ __launch_bounds__(kThreads) void paged_sums_kernel(const PagedAttnArgs a) {
+  const int chunks = (a.max_units * kPagedUnit + kSumKeys - 1) / kSumKeys;
+  const int chunk = blockIdx.x % chunks, stream = blockIdx.x / chunks, hkv = stream % a.c.Hkv, b = stream / a.c.Hkv;
+  const Visible vis = visible(seq_len(a.c, b), a.W, a.S);
+  const int end = imin(vis.count, (chunk + 1) * kSumKeys);
+  for (int v = chunk * kSumKeys + threadIdx.x; v < end; v += kThreads) {
+    const float* x = a.logits + ((int64_t(hkv) * a.c.B + b) * a.max_units + v / kPagedUnit) * a.G * kPagedUnit + v % kPagedUnit;
+    const float* lse = a.lse + int64_t(b) * a.Hq + hkv * a.G;
+    float w = 0.f;
+    for (int g = 0; g < a.G; ++g) {
+      const float s = x[g * kPagedUnit];
+      w += s == kNegInf ? 0.f : fast_exp2(s - lse[g]);
+    }
+    a.sums[int64_t(b) * a.ssum[0] + int64_t(hkv) * a.ssum[1] + visible_key(vis, v)] += w;
+  }
+}
+
+template <typename E, int D>
+hipError_t run(const PagedAttnArgs& a, hipStream_t s) {
+  const int streams = a.c.Hkv * a.row_tiles;
+  hipLaunchKernelGGL((paged_attn_kernel<E, D>), dim3(unsigned(streams) * unsigned(a.parts ? a.parts : a.c.B)), dim3(kThreads), 0, s, a);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  if (a.parts) {
+    hipLaunchKernelGGL((paged_join_kernel<E, D>), dim3(unsigned(a.Hq) * unsigned(a.c.B)), dim3(64), 0, s, a);
+    e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  if (a.sums) {
+    const unsigned chunks = unsigned((a.max_units * kPagedUnit + kSumKeys - 1) / kSumKeys);
+    hipLaunchKernelGGL(paged_sums_kernel, dim3(chunks * unsigned(a.c.Hkv) * unsigned(a.c.B)), dim3(kThreads), 0, s, a);
+    e = hipGetLastError();
+  }
+  return e;
+}
+
+template <typename E>
+hipError_t run_d(const PagedAttnArgs& a, int D, hipStream_t s) {
+  if constexpr (E::CB == 1) return D == 64 ? run<E, 64>(a, s) : run<E, 128>(a, s);
+  else return D == 16 ? run<E, 16>(a, s) : D == 32 ? run<E, 32>(a, s) : D == 64 ? run<E, 64>(a, s) : run<E, 128>(a, s);
+}
+
+}  // namespace
+
+hipError_t launch_paged_attention(const PagedAttnArgs& a, int dtype, int cache, int D, hipStream_t s) {
+  if (dtype == FA_DTYPE_F32) return run_d<PF32>(a, D, s);
+  if (dtype == FA_DTYPE_BF16) return cache == FA_DTYPE_FP8_E4M3 ? run_d<PBF16Q8>(a, D, s) : run_d<PBF16>(a, D, s);
+  return cache == FA_DTYPE_FP8_E4M3 ? run_d<PF16Q8>(a, D, s) : run_d<PF16>(a, D, s);
+}
+
+}  // namespace fa

@@ -496,9 +496,231 @@ py::object quantize_fp8(const at::Tensor& x_in, c10::optional<double> descale) {
   return py::make_tuple(x8, amax > 0.f ? double(amax) / 448.0 : 1.0);
 }
 
+// ---- paged key-value caches --------------------------------------------------------------------
+// The calls of paged.py.  They write tensors of their caller in place, which no trace or transform can see.
+void refuse_transformed(std::initializer_list<const at::Tensor*> ts, const char* what) {
+  if (transformed(ts))
+    throw std::runtime_error(std::string(what) + " works on tensors in place: it cannot be traced or transformed");
+}
+
+std::string shape_of(const at::Tensor& t) {
+  std::string r = "[";
+  for (int64_t i = 0; i < t.dim(); ++i) r += (i ? ", " : "") + std::to_string(t.size(i));
+  return r + "]";
+}
+
+void on_device(const at::Tensor& t, const at::Tensor& first, const char* name, const char* first_name) {
+  if (t.device() != first.device())
+    throw std::runtime_error(std::string(name) + " is on " + t.device().str() + " but " + first_name + " is on " +
+                             first.device().str());
+}
+
+int32_t to_i32(int64_t x, const char* name) {
+  if (x < INT32_MIN || x > INT32_MAX) throw std::invalid_argument(std::string(name) + " does not fit 32 bits");
+  return int32_t(x);
+}
+
+// What a call changed in place, as far as autograd's version counters go.
+void changed(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
+// The cache's parameter block.  block_table and lens are copied where their entries are not next to each other; the copies
+// are kept in `keep` for the call.
+fa_paged_cache paged_cache(const at::Tensor& k_pages, const at::Tensor& v_pages, const at::Tensor& table,
+                           const at::Tensor& lens, double k_descale, double v_descale, std::vector<at::Tensor>& keep) {
+  if (!k_pages.is_cuda())
+    throw std::runtime_error("k_pages is on " + k_pages.device().str() +
+                             ": the gfx950 attention kernels need GPU tensors (there is no CPU implementation)");
+  on_device(v_pages, k_pages, "v_pages", "k_pages");
+  on_device(table, k_pages, "block_table", "k_pages");
+  on_device(lens, k_pages, "lens", "k_pages");
+  if (k_pages.dim() != 4 || v_pages.sizes() != k_pages.sizes())
+    throw std::invalid_argument("k_pages and v_pages must both be [pages, Hkv, page_size, D], got " + shape_of(k_pages) + " and " +
+                                shape_of(v_pages));
+  if (v_pages.scalar_type() != k_pages.scalar_type()) throw std::invalid_argument("v_pages has a different dtype than k_pages");
+  fa_paged_cache c{};
+  if (k_pages.scalar_type() == at::kFloat8_e4m3fn) c.dtype = FA_DTYPE_FP8_E4M3;
+  else if (k_pages.scalar_type() == at::kBFloat16) c.dtype = FA_DTYPE_BF16;
+  else if (k_pages.scalar_type() == at::kHalf) c.dtype = FA_DTYPE_F16;
+  else if (k_pages.scalar_type() == at::kFloat) c.dtype = FA_DTYPE_F32;
+  else
+    throw std::invalid_argument("k_pages has dtype " + std::string(c10::toString(k_pages.scalar_type())) +
+                                "; supported dtypes are bfloat16, float16, float32 and float8_e4m3fn");
+  if (c.dtype != FA_DTYPE_FP8_E4M3 && (k_descale != 1.0 || v_descale != 1.0))
+    throw std::invalid_argument("descale is for float8_e4m3fn pages only");
+  if (k_pages.numel() == 0) throw std::invalid_argument("k_pages must not be empty, got " + shape_of(k_pages));
+  for (const at::Tensor* t : {&k_pages, &v_pages}) {
+    const int64_t m = 16 / int64_t(t->element_size()) - 1;
+    if (t->stride(3) != 1 || (t->stride(0) & m) || (t->stride(1) & m) || (t->stride(2) & m) ||
+        (reinterpret_cast<uintptr_t>(t->data_ptr()) & 15))
+      throw std::invalid_argument("pages are used in place: their head-dim stride must be 1, the other strides multiples of 16 "
+                                  "bytes and their base 16-byte aligned");
+  }
+  if (table.dim() != 2 || table.scalar_type() != at::kInt || table.size(0) < 1 || table.size(1) < 1)
+    throw std::invalid_argument("block_table must be int32 [B, width], got " + shape_of(table));
+  if (lens.dim() != 1 || lens.scalar_type() != at::kInt || lens.size(0) != table.size(0))
+    throw std::invalid_argument("lens must be int32 [B] with the block_table's B, got " + shape_of(lens));
+  keep.push_back(table.stride(1) == 1 || table.size(1) == 1 ? table : table.contiguous());
+  c.table = keep.back().data_ptr<int32_t>();
+  c.table_stride = keep.back().stride(0);
+  keep.push_back(lens.contiguous());
+  c.lens = keep.back().data_ptr<int32_t>();
+  c.k = k_pages.data_ptr();
+  c.v = v_pages.data_ptr();
+  strides3(c.k_stride, k_pages);
+  strides3(c.v_stride, v_pages);
+  c.batch = to_i32(table.size(0), "the batch");
+  c.table_width = to_i32(table.size(1), "the block_table's width");
+  c.pages = to_i32(k_pages.size(0), "the number of pages");
+  c.heads_kv = to_i32(k_pages.size(1), "the number of heads");
+  c.page_size = to_i32(k_pages.size(2), "the page size");
+  c.head_dim = to_i32(k_pages.size(3), "the head dim");
+  c.k_descale = k_descale;
+  c.v_descale = v_descale;
+  return c;
+}
+
+// A [rows, H, D] input of a call: of one 16- or 32-bit type, copied where the kernels cannot read it.
+at::Tensor paged_input(const at::Tensor& t, const at::Tensor& k_pages, const char* name) {
+  on_device(t, k_pages, name, "k_pages");
+  const bool e4m3 = k_pages.scalar_type() == at::kFloat8_e4m3fn;
+  if (t.dim() != 3 || t.size(2) != k_pages.size(3))
+    throw std::invalid_argument(std::string(name) + " must be 3-D with the pages' head dim " + std::to_string(k_pages.size(3)) +
+                                ", got " + shape_of(t));
+  if (e4m3 ? t.scalar_type() != at::kBFloat16 && t.scalar_type() != at::kHalf : t.scalar_type() != k_pages.scalar_type())
+    throw std::invalid_argument(std::string(name) + " has dtype " + c10::toString(t.scalar_type()) + " over pages of " +
+                                c10::toString(k_pages.scalar_type()) +
+                                "; both must have the same type, or bfloat16 or float16 over float8_e4m3fn pages");
+  const int64_t m = 16 / int64_t(t.element_size()) - 1;
+  if (t.stride(2) != 1 || (t.stride(0) & m) || (t.stride(1) & m) || (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15))
+    return t.clone(at::MemoryFormat::Contiguous);
+  return t;
+}
+
+void paged_append(const at::Tensor& k_in, const at::Tensor& v_in, const at::Tensor& k_pages, const at::Tensor& v_pages,
+                  const at::Tensor& table, const at::Tensor& lens, const c10::optional<at::Tensor>& cu, double k_descale,
+                  double v_descale) {
+  refuse_transformed({&k_in, &v_in, &k_pages, &v_pages}, "paged_append");
+  std::vector<at::Tensor> keep;
+  const fa_paged_cache c = paged_cache(k_pages, v_pages, table, lens, k_descale, v_descale, keep);
+  const c10::DeviceGuard guard(k_pages.device());
+  const at::Tensor k = paged_input(k_in, k_pages, "k"), v = paged_input(v_in, k_pages, "v");
+  if (k.size(1) != k_pages.size(1) || v.sizes() != k.sizes() || v.scalar_type() != k.scalar_type())
+    throw std::invalid_argument("k and v must both be [rows, Hkv, D] of one dtype, got " + shape_of(k) + " and " + shape_of(v));
+  const bool packed = cu.has_value();
+  if (packed && (cu->device() != k.device() || cu->scalar_type() != at::kInt || cu->dim() != 1 || !cu->is_contiguous() ||
+                 cu->size(0) != table.size(0) + 1))
+    throw std::invalid_argument("cu_seqlens must hold B + 1 offsets, got " + shape_of(*cu));
+  if (!packed && k.size(0) != table.size(0))
+    throw std::invalid_argument("without cu_seqlens k and v have one row a sequence, got " + shape_of(k));
+  const int64_t ks[2] = {k.stride(1), k.stride(0)}, vs[2] = {v.stride(1), v.stride(0)};
+  raise_for_status(fa_paged_append(&c, k.data_ptr(), v.data_ptr(), ks, vs, to_i32(k.size(0), "the number of rows"), dtype_code(k),
+                                   packed ? cu->data_ptr<int32_t>() : nullptr, current_stream(k)),
+                   "fa_paged_append");
+  changed(k_pages);
+  changed(v_pages);
+}
+
+at::Tensor paged_attention(const at::Tensor& q_in, const at::Tensor& k_pages, const at::Tensor& v_pages,
+                           const at::Tensor& table, const at::Tensor& lens, int64_t window, int64_t sink,
+                           const c10::optional<at::Tensor>& sinks_in, double scale, double k_descale, double v_descale,
+                           int64_t max_len, const c10::optional<at::Tensor>& sums) {
+  refuse_transformed({&q_in, &k_pages, &v_pages}, "paged_attention");
+  std::vector<at::Tensor> keep;
+  fa_paged_attention_params p{};
+  p.cache = paged_cache(k_pages, v_pages, table, lens, k_descale, v_descale, keep);
+  const c10::DeviceGuard guard(k_pages.device());
+  const at::Tensor q = paged_input(q_in, k_pages, "q");
+  const int64_t B = table.size(0), Hq = q.size(1);
+  if (q.size(0) != B || Hq < 1 || Hq % k_pages.size(1) != 0)
+    throw std::invalid_argument("q must be [B, Hq, D] with the block_table's B and a multiple of the pages' heads, got " + shape_of(q));
+  const at::Tensor sinks = sinks_in.has_value() ? sinks_ready(*sinks_in, Hq, q) : at::Tensor();
+  at::Tensor o = at::empty({B, Hq, q.size(2)}, q.options());
+  p.q = q.data_ptr();
+  p.o = o.data_ptr();
+  p.q_stride[0] = q.stride(0);
+  p.q_stride[1] = q.stride(1);
+  p.o_stride[0] = o.stride(0);
+  p.o_stride[1] = o.stride(1);
+  p.sinks = sinks.defined() ? sinks.data_ptr<float>() : nullptr;
+  if (sums.has_value()) {
+    on_device(*sums, k_pages, "weight_sums", "k_pages");
+    if (sums->scalar_type() != at::kFloat || sums->dim() != 3 || sums->size(0) != B || sums->size(1) != k_pages.size(1) ||
+        (sums->stride(2) != 1 && sums->size(2) != 1))
+      throw std::invalid_argument("weight_sums must be float32 [B, Hkv, tokens], next to each other in the last dimension, got " +
+                                  shape_of(*sums));
+    p.weight_sums = sums->data_ptr<float>();
+    p.sums_stride[0] = sums->stride(0);
+    p.sums_stride[1] = sums->stride(1);
+    p.sums_width = clamp_i32(sums->size(2));
+  }
+  p.heads_q = to_i32(Hq, "the number of heads");
+  p.max_len = clamp_i32(max_len);
+  p.window = clamp_i32(window);
+  p.sink = clamp_i32(sink);
+  p.dtype = dtype_code(q);
+  p.softmax_scale = float(scale);
+  const size_t bytes = fa_paged_workspace_bytes(&p);
+  at::Tensor ws = at::empty({int64_t(bytes > 256 ? bytes : 256)}, q.options().dtype(at::kByte));
+  raise_for_status(fa_paged_attention(&p, ws.data_ptr(), size_t(ws.numel()), current_stream(q)), "fa_paged_attention");
+  if (sums.has_value()) changed(*sums);
+  return o;
+}
+
+// (new lens, new weight sums)
+std::vector<at::Tensor> paged_evict(const at::Tensor& k_pages, const at::Tensor& v_pages, const at::Tensor& table,
+                                    const at::Tensor& lens, const at::Tensor& sums, int64_t kept, const at::Tensor& new_table_in,
+                                    int64_t sink, int64_t recent) {
+  refuse_transformed({&k_pages, &v_pages, &sums}, "paged_evict");
+  std::vector<at::Tensor> keep;
+  fa_paged_evict_params p{};
+  p.cache = paged_cache(k_pages, v_pages, table, lens, 1.0, 1.0, keep);
+  const c10::DeviceGuard guard(k_pages.device());
+  on_device(sums, k_pages, "weight_sums", "k_pages");
+  on_device(new_table_in, k_pages, "new_table", "k_pages");
+  const int64_t B = table.size(0), Hkv = k_pages.size(1);
+  if (sums.scalar_type() != at::kFloat || sums.dim() != 3 || sums.size(0) != B || sums.size(1) != Hkv ||
+      (sums.stride(2) != 1 && sums.size(2) != 1))
+    throw std::invalid_argument("weight_sums must be float32 [B, Hkv, tokens], next to each other in the last dimension, got " +
+                                shape_of(sums));
+  if (new_table_in.dim() != 2 || new_table_in.scalar_type() != at::kInt || new_table_in.size(0) != B || new_table_in.size(1) < 1)
+    throw std::invalid_argument("new_table must be int32 [B, width], got " + shape_of(new_table_in));
+  if (new_table_in.data_ptr() == table.data_ptr())
+    throw std::invalid_argument("new_table must name other pages than block_table");
+  const at::Tensor new_table = new_table_in.stride(1) == 1 || new_table_in.size(1) == 1 ? new_table_in : new_table_in.contiguous();
+  at::Tensor new_lens = at::empty({B}, lens.options());
+  at::Tensor new_sums = at::empty({B, Hkv, sums.size(2)}, sums.options());
+  p.sums = sums.data_ptr<float>();
+  p.new_sums = new_sums.data_ptr<float>();
+  for (int i = 0; i < 2; ++i) {
+    p.sums_stride[i] = sums.stride(i);
+    p.new_sums_stride[i] = new_sums.stride(i);
+  }
+  p.sums_width = clamp_i32(sums.size(2));
+  p.new_table = new_table.data_ptr<int32_t>();
+  p.new_table_stride = new_table.stride(0);
+  p.new_table_width = to_i32(new_table.size(1), "the new_table's width");
+  p.new_lens = new_lens.data_ptr<int32_t>();
+  p.keep = to_i32(kept, "keep");
+  p.sink = to_i32(sink, "sink_size");
+  p.recent = to_i32(recent, "recent");
+  const size_t bytes = fa_paged_evict_workspace_bytes(p.cache.batch, p.cache.heads_kv, p.keep);
+  at::Tensor ws = at::empty({int64_t(bytes > 256 ? bytes : 256)}, sums.options().dtype(at::kByte));
+  raise_for_status(fa_paged_evict(&p, ws.data_ptr(), size_t(ws.numel()), current_stream(sums)), "fa_paged_evict");
+  changed(k_pages);
+  changed(v_pages);
+  return {new_lens, new_sums};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+  m.def("paged_append", &paged_append, "(k, v, k_pages, v_pages, block_table, lens, cu_seqlens, k_descale, v_descale)");
+  m.def("paged_attention", &paged_attention,
+        "(q, k_pages, v_pages, block_table, lens, window, sink, sinks, scale, k_descale, v_descale, max_len, weight_sums) -> o");
+  m.def("paged_evict", &paged_evict,
+        "(k_pages, v_pages, block_table, lens, weight_sums, keep, new_table, sink, recent) -> (new lens, new weight sums)");
   m.def("swda", &swda,
         "autograd forward of causal sliding-window + sink attention: (q, k, v, window, sink, scale) -> o or None",
         py::arg("q"), py::arg("k"), py::arg("v"), py::arg("window"), py::arg("sink"), py::arg("scale"));

@@ -61,7 +61,9 @@ enum fa_status {
   FA_ERR_LAUNCH = -8,      /* a HIP launch failed */
   FA_ERR_OVERFLOW = -9,    /* a size or element offset does not fit the kernels' index math */
   FA_ERR_SCALE = -10,      /* softmax_scale is NaN or infinite */
-  FA_ERR_SCRATCH = -11     /* fa_bwd_scratch: the problem needs more workspace than FA_SCRATCH_BYTES */
+  FA_ERR_SCRATCH = -11,    /* fa_bwd_scratch: the problem needs more workspace than FA_SCRATCH_BYTES */
+  FA_ERR_PAGES = -12       /* paged caches: pages, page size or table width < 1, or a size that does not cover the
+                              table's tokens (weight sums), the kept entries (new table) or the protected ones (keep) */
 };
 
 /* Size of the library's own device scratch buffer used by fa_bwd_scratch (per GPU). */
@@ -258,6 +260,82 @@ int fa_fwd_fp8(const fa_fwd_params* p, float q_descale, float k_descale, float v
  * fa_fwd_fp8 (none: flash_attention_gpt_oss.py:356-383 takes 16/32-bit tensors only). */
 int fa_fwd_fp8_pv(const fa_fwd_params* p, float q_descale, float k_descale, float v_descale, const float* sinks,
                   void* stream);
+
+/* Paged key-value caches, for answering with a model: one new token a sequence at a time against the keys and values
+ * of all tokens before it.  The reference has no counterpart (its kernels take whole sequences,
+ * flash_attention_gpt_oss.py:348).  A layer's cache is a pool of pages of page_size entries; row b of the table
+ * lists the pages of sequence b in order, so token t of the sequence lies on page table[b][t / page_size] in slot
+ * t % page_size.  Any order of head and slot in memory is described by the strides.
+ *   - table (int32 [batch][table_width]) and lens (int32 [batch], tokens of each sequence) are in DEVICE memory, so the
+ *     library cannot check them.  Lengths are cut off to [0, table_width * page_size]; an entry outside [0, pages) is no
+ *     page: nothing is written there, and its tokens count as masked.  So bad values stay inside the tensors.
+ *   - dtype: the pages' type, that of the call's other tensors or FA_DTYPE_FP8_E4M3 (head_dim 64 or 128) under bf16 or fp16
+ *     tensors; an e4m3 code stands for k_descale (v_descale) times its value.  Other types ignore the descales. */
+typedef struct fa_paged_cache {
+  void* k;                /* [pages, Hkv, page_size, D] */
+  void* v;
+  int64_t k_stride[3];    /* page, head, slot strides in elements: multiples of 16 bytes */
+  int64_t v_stride[3];
+  const int32_t* table;
+  const int32_t* lens;
+  int64_t table_stride;   /* entries between the table's rows */
+  int32_t batch, pages, page_size, table_width, heads_kv, head_dim;
+  int32_t dtype;          /* enum fa_dtype */
+  double k_descale, v_descale;
+} fa_paged_cache;
+
+/* Writes new tokens' rows into the cache.  k, v: [rows, Hkv, D] of type `dtype`, strides (head, row) in elements.
+ * Sequence b's rows are [cu_seqlens[b], cu_seqlens[b + 1]) (int32 [batch + 1] in device memory), or row b where
+ * cu_seqlens is NULL (rows = batch).  lens count the new tokens already: the n rows of sequence b go to its positions
+ * lens[b] - n .. lens[b] - 1.  Rows of no sequence and of positions outside the table are left out (lens[b] = 0: an
+ * idle sequence of a decoding batch).  e4m3 pages get the codes of clamp(x / descale, -448, 448), dividing as a product with
+ * the reciprocal of descale rounded to float32.  Two sequences must not write the same entry. */
+int fa_paged_append(const fa_paged_cache* c, const void* k, const void* v, const int64_t k_stride[2],
+                    const int64_t v_stride[2], int32_t rows, int32_t dtype, const int32_t* cu_seqlens, void* stream);
+
+/* Attention of the last token of every sequence over its cache: query head h of sequence b sees key k < lens[b] where
+ * lens[b] - 1 - k < window or k < sink.  Learned sinks (float32 [Hq]) are optional (NULL), as in fa_fwd_sinks.  A sequence
+ * that sees no key gets o = 0.  With weight_sums (float32 [batch, Hkv, at least min(max_len, table tokens)], NULL: none) the
+ * softmax weights are accumulated: weight_sums[b, h, k] += sum over the query heads of KV head h of P[k], in a fixed
+ * order.  max_len bounds lens (they are cut off there); it and the table's width size the grid and the workspace, of
+ * which at least fa_paged_workspace_bytes() are needed, 256-byte aligned. */
+typedef struct fa_paged_attention_params {
+  fa_paged_cache cache;
+  const void* q;          /* [batch, Hq, D] */
+  void* o;                /* [batch, Hq, D] */
+  int64_t q_stride[2];    /* batch, head */
+  int64_t o_stride[2];
+  const float* sinks;
+  float* weight_sums;
+  int64_t sums_stride[2]; /* batch, KV head */
+  int32_t sums_width;     /* entries of a (sequence, KV head) in weight_sums */
+  int32_t heads_q, max_len, window, sink;
+  int32_t dtype;          /* of q and o */
+  float softmax_scale;
+} fa_paged_attention_params;
+size_t fa_paged_workspace_bytes(const fa_paged_attention_params* p); /* 0 for an invalid problem */
+int fa_paged_attention(const fa_paged_attention_params* p, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Eviction by accumulated attention weight.  Every sequence of n > keep tokens is thinned out to keep entries, each KV
+ * head by itself: the first `sink` and the last `recent` entries stay, and of the others those with the largest
+ * weight_sums, the lower position first among equals (a NaN counts as the largest).  Kept entries go, in order, to
+ * positions 0, 1, ... of the pages of new_table ([batch][new_table_width]), which must not be pages that the call reads;
+ * shorter sequences are copied whole.  new_sums gets the kept entries' sums and zeros behind them, new_lens
+ * min(n, keep).  Positions have no meaning for the window or the sinks of an attention call any more.  The
+ * workspace holds at least fa_paged_evict_workspace_bytes(batch, heads_kv, keep). */
+typedef struct fa_paged_evict_params {
+  fa_paged_cache cache;
+  const float* sums;      /* [batch, Hkv, sums_width] */
+  float* new_sums;
+  int64_t sums_stride[2]; /* batch, KV head */
+  int64_t new_sums_stride[2];
+  const int32_t* new_table;
+  int64_t new_table_stride;
+  int32_t* new_lens;      /* [batch] */
+  int32_t sums_width, new_table_width, keep, sink, recent;
+} fa_paged_evict_params;
+size_t fa_paged_evict_workspace_bytes(int32_t batch, int32_t heads_kv, int32_t keep);
+int fa_paged_evict(const fa_paged_evict_params* p, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Host-only argument checks used by fa_fwd / fa_bwd (no HIP call is made). */
 int fa_check_fwd(const fa_fwd_params* p);
