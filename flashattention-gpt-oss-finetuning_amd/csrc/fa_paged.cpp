@@ -70,6 +70,9 @@ constexpr int kWholeKeys = 512;
 // Workgroups of a split call's launch for each compute unit, and the fewest units worth a workgroup of their own.
 constexpr int kPartsPerCu = 2, kLeastUnits = 2;
 
+// K and V bytes up to which a call's loads leave them in the 256 MB last-level cache, for the next step to find.
+constexpr int64_t kKeepBytes = int64_t(96) << 20;
+
 struct Plan {
   int max_units, row_tiles, parts;
   size_t part_o, part_ml, lse, logits;  // bytes
@@ -106,7 +109,8 @@ int plan(const fa_paged_attention_params* p, Plan* r) {
   r->parts = 0;
   if (most > kWholeKeys) {
     const int64_t want = std::max<int64_t>(1, int64_t(kPartsPerCu) * fa::device_cus() / streams);
-    r->parts = int(std::min(want, (units + kLeastUnits - 1) / kLeastUnits));
+    // (whole rounds of the 8 XCDs: the tiles of a group's heads then read the same keys through one L2)
+    r->parts = int((std::min(want, (units + kLeastUnits - 1) / kLeastUnits) + 7) / 8 * 8);
     if (!fa::grid_fits(streams * r->parts)) return FA_ERR_OVERFLOW;
   }
   const size_t slots = size_t(streams) * r->parts * 2;
@@ -116,8 +120,8 @@ int plan(const fa_paged_attention_params* p, Plan* r) {
   if (p->weight_sums) {
     r->lse = align256(size_t(c.batch) * p->heads_q * sizeof(float));
     r->logits = align256(size_t(units) * p->heads_q * fa::kPagedUnit * sizeof(float));
-    // (the launch that adds up the weights: a workgroup for 1024 keys, at least one a (sequence, KV head))
-    if (!fa::grid_fits((r->max_units + 7) / 8 * int64_t(c.heads_kv) * c.batch)) return FA_ERR_OVERFLOW;
+    // (the second launch: a workgroup a query head, and one for each 1024 keys of a (sequence, KV head))
+    if (!fa::grid_fits((p->heads_q + int64_t(r->max_units + 7) / 8 * c.heads_kv) * c.batch)) return FA_ERR_OVERFLOW;
   }
   return FA_OK;
 }
@@ -193,6 +197,7 @@ int fa_paged_attention(const fa_paged_attention_params* p, void* workspace, size
   a.max_units = r.max_units;
   a.parts = r.parts;
   a.least = kLeastUnits;
+  a.keep_units = int(std::min<int64_t>(kKeepBytes / (int64_t(fa::kPagedUnit) * 2 * c.head_dim * elem_bytes(c.dtype) * c.heads_kv), INT32_MAX));
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   a.part_o = reinterpret_cast<float*>(ws);
   a.part_ml = reinterpret_cast<float*>(ws + r.part_o);

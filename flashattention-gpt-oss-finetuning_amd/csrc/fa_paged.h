@@ -46,10 +46,11 @@ struct PagedAttnArgs {
   int max_units;          // units of a sequence of max_len tokens
   // split calls: the runs a (KV head, row tile) is cut into, 0 where every workgroup takes a whole sequence
   int parts, least;
+  int keep_units;         // calls that read more units a KV head than this mark their loads as read once
   // workspace
   float* part_o;          // [Hkv row_tiles][parts][2][16][D]
   float* part_ml;         // [Hkv row_tiles][parts][2][2][16]: maximum (log2 domain), sum
-  float* lse;             // with sums: [B][Hq] (log2 domain)
+  float* lse;             // with sums: [B][Hq] (log2 domain), of the sequences that one workgroup took whole
   float* logits;          // with sums: [Hkv][B][max_units][G][kPagedUnit] (log2 domain)
 };
 

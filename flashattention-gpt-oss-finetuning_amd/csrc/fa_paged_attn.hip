@@ -19,15 +19,15 @@
 // P goes into the 16-bit product as the sum of two 16-bit parts (P rounded, and what that left), so o carries its own
 // rounding only; the second product costs matrix time that the loads leave idle.  float32 uses v_mfma_f32_16x16x4.
 //
-// Keys are addressed through an LDS table of 64-bit offsets, filled for 512 keys at a time: key -> page -> offset is
-// worked out once a key.  A key on no page (an entry outside [0, pages)) and the keys past the end have offset -1; their
-// scores become -inf and their V entries 0, whatever lies in memory.
+// Keys are addressed through a wave's own LDS table of 64-bit offsets, 64 keys at a time: key -> page -> offset is worked
+// out once a key, ahead of its use.  Keys on no page (an entry outside [0, pages)) and those past the end are marked in a
+// mask; their scores become -inf and their V entries 0, whatever lies in memory (they are loaded from entry 0 of page 0).
 //
 // Runs.  With a workgroup a (KV head, sequence) long sequences would leave the chip idle, and with a fixed number of
 // pieces a sequence ragged batches would.  Split calls deal out the units of all sequences evenly
 // (fa_paged_plan.h): each workgroup finds its run by a prefix sum over lens, on the device, so the grid depends on
 // sizes the host knows.  Pieces that are no whole sequence leave (maximum, sum, o) in the workspace, and
-// paged_join_kernel adds them in order.
+// paged_finish_kernel joins them.
 #include <hip/hip_runtime.h>
 
 #include "../../include/fa_gfx950.h"
@@ -40,7 +40,6 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWaves = 4;
 constexpr int kTile = 32;
-constexpr int kFill = 512;  // keys of an LDS offset table
 
 __device__ __forceinline__ int seq_len(const PagedCache& c, int b) { return imin(imax(c.lens[b], 0), c.max_len); }
 
@@ -123,16 +122,25 @@ __device__ __forceinline__ float quarters_sum(float x) {
   return x + __shfl_xor(x, 32);
 }
 
+template <bool ONCE, typename T>
+__device__ __forceinline__ T fetch(const T* p) {
+  if constexpr (ONCE) return __builtin_nontemporal_load(p);
+  else return *p;
+}
+
 // One wave's tile of 32 keys in registers.
 template <typename E, int D>
 struct Tile {
   static constexpr int ROW = D * E::CB;                      // bytes of an entry
-  static constexpr int NK = ROW >= 64 ? ROW / 64 : 1;        // 16-byte pieces of an entry that a lane holds
+  static constexpr int PR = ROW / 16;                        // 16-byte pieces of an entry
+  static constexpr int NF = PR >= 4 ? PR / 4 : 1;            // of those that a lane supplies to the products
+  static constexpr bool STAGED = E::CB < 4;                  // K goes through LDS
+  static constexpr int NK = STAGED ? PR / 2 : 2 * NF;        // pieces of the tile that a lane loads
   static constexpr int VB = ROW / 16;                        // bytes of a V entry that a lane holds
   static constexpr int VD = VB >= 4 ? VB / 4 : 1;
-  u32x4 k[2][NK];
+  u32x4 k[NK];
   uint32_t v[8][VD];
-  bool gone;  // some key of the tile is on no page or past the end
+  uint32_t live;  // bit i: key i of the tile is on a page (the same in every lane)
 };
 
 template <typename E, int D>
@@ -163,40 +171,44 @@ struct Wave {
     l = 0.f;
   }
 
-  // off: the tile's 32 offsets of K, and of V, in LDS.
-  static __device__ __forceinline__ void load(T& t, const uint8_t* k, const uint8_t* v, const int64_t* koff, const int64_t* voff) {
+  // koff, voff: the tile's 32 offsets of K, and of V, in LDS.
+  template <bool ONCE>
+  static __device__ __forceinline__ void load(T& t, const uint8_t* k, const uint8_t* v, const int64_t* koff, const int64_t* voff,
+                                              uint32_t live) {
     const int lane = threadIdx.x & 63, r = lane & 15, j = lane >> 4;
+    t.live = live;
+    if constexpr (T::STAGED) {  // neighbouring lanes take neighbouring pieces
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int64_t o = koff[8 * (r >> 2) + 4 * h + (r & 3)];
-      const uint8_t* p = k + (o < 0 ? 0 : o);
+      for (int n = 0; n < T::NK; ++n)
+        t.k[n] = fetch<ONCE>(reinterpret_cast<const u32x4*>(k + koff[(64 * n + lane) / T::PR] + 16 * (lane % T::PR)));
+    } else {
 #pragma unroll
-      for (int n = 0; n < T::NK; ++n) t.k[h][n] = 64 * n + 16 * j < T::ROW ? ld16(p + 64 * n + 16 * j) : zero16();
+      for (int h = 0; h < 2; ++h) {
+        const uint8_t* p = k + koff[8 * (r >> 2) + 4 * h + (r & 3)];
+#pragma unroll
+        for (int n = 0; n < T::NF; ++n) t.k[h * T::NF + n] = fetch<ONCE>(reinterpret_cast<const u32x4*>(p + 64 * n + 16 * j));
+      }
     }
-    bool gone = false;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const int64_t o = voff[8 * j + e];
-      gone |= o < 0;
-      const uint8_t* p = v + (o < 0 ? 0 : o) + T::VB * r;
+      const uint8_t* p = v + voff[8 * j + e] + T::VB * r;
       if constexpr (T::VB == 2) {
-        t.v[e][0] = *reinterpret_cast<const uint16_t*>(p);
+        t.v[e][0] = fetch<ONCE>(reinterpret_cast<const uint16_t*>(p));
       } else if constexpr (T::VB == 4) {
-        t.v[e][0] = *reinterpret_cast<const uint32_t*>(p);
+        t.v[e][0] = fetch<ONCE>(reinterpret_cast<const uint32_t*>(p));
       } else if constexpr (T::VB == 8) {
-        const u32x2 x = *reinterpret_cast<const u32x2*>(p);
+        const u32x2 x = fetch<ONCE>(reinterpret_cast<const u32x2*>(p));
         t.v[e][0] = x[0];
         t.v[e][1] = x[1];
       } else {
 #pragma unroll
         for (int w = 0; w < T::VB / 16; ++w) {
-          const u32x4 x = ld16(p + 16 * w);
+          const u32x4 x = fetch<ONCE>(reinterpret_cast<const u32x4*>(p + 16 * w));
 #pragma unroll
           for (int i = 0; i < 4; ++i) t.v[e][4 * w + i] = x[i];
         }
       }
     }
-    t.gone = wave_any(gone);
   }
 
   // Eight keys' values of dim c of this lane as an A operand: v[e] holds D / 16 dims of key 8j + e.
@@ -208,39 +220,62 @@ struct Wave {
     return f;
   }
 
-  // voff: the tile's offsets (for tiles with keys that do not count); logits: where the lane's eight scores go, or NULL
-  __device__ __forceinline__ void step(T& t, float c2, const int64_t* voff, float* logits) {
-    const int lane = threadIdx.x & 63, j = lane >> 4;
+  // Place of piece p of the tile's key row in the staged tile: the rows 0..3 and 8..11 (and 4 or 16 more) that eight lanes
+  // read at once, at the same piece, get different banks.
+  static __device__ __forceinline__ int staged(int row, int p) {
+    constexpr int PR = T::PR;
+    const int s = PR >= 8 ? (row & 3) | (row >> 1 & 4) : PR == 4 ? (row >> 1 & 1) | (row >> 2 & 2) : row >> 3 & 1;
+    return row * PR + (p ^ s);
+  }
+
+  // lds: the wave's room for a staged K tile; logits: where the lane's eight scores go, or NULL
+  __device__ __forceinline__ void step(T& t, float c2, u32x4* lds, float* logits) {
+    const int lane = threadIdx.x & 63, r = lane & 15, j = lane >> 4;
     f32x4 s0 = {0.f, 0.f, 0.f, 0.f}, s1 = s0;
+    u32x4 kf[2][T::NF];
+    if constexpr (T::STAGED) {
+#pragma unroll
+      for (int n = 0; n < T::NK; ++n) lds[staged((64 * n + lane) / T::PR, lane % T::PR)] = t.k[n];
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int n = 0; n < T::NF; ++n)
+          kf[h][n] = 4 * n + j < T::PR ? lds[staged(8 * (r >> 2) + 4 * h + (r & 3), 4 * n + j)] : zero16();
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    } else {
+#pragma unroll
+      for (int n = 0; n < 2 * T::NF; ++n) kf[n / T::NF][n % T::NF] = t.k[n];
+    }
     if constexpr (F) {
 #pragma unroll
-      for (int n = 0; n < T::NK; ++n)
+      for (int n = 0; n < T::NF; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const uint32_t k0 = t.k[0][n][e], k1 = t.k[1][n][e], qe = q[n][e];
+          const uint32_t k0 = kf[0][n][e], k1 = kf[1][n][e], qe = q[n][e];
           s0 = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, k0), __builtin_bit_cast(float, qe), s0, 0, 0, 0);
           s1 = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, k1), __builtin_bit_cast(float, qe), s1, 0, 0, 0);
         }
     } else {
 #pragma unroll
-      for (int n = 0; n < T::NK; ++n) {
+      for (int n = 0; n < T::NF; ++n) {
         if constexpr (E::CB == 1) {
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
             u32x4 k0, k1;
 #pragma unroll
             for (int w = 0; w < 2; ++w) {
-              k0[2 * w] = E::widen(t.k[0][n][2 * u + w], false);
-              k0[2 * w + 1] = E::widen(t.k[0][n][2 * u + w], true);
-              k1[2 * w] = E::widen(t.k[1][n][2 * u + w], false);
-              k1[2 * w + 1] = E::widen(t.k[1][n][2 * u + w], true);
+              k0[2 * w] = E::widen(kf[0][n][2 * u + w], false);
+              k0[2 * w + 1] = E::widen(kf[0][n][2 * u + w], true);
+              k1[2 * w] = E::widen(kf[1][n][2 * u + w], false);
+              k1[2 * w + 1] = E::widen(kf[1][n][2 * u + w], true);
             }
             s0 = E::mfma16(k0, q[2 * n + u], s0);
             s1 = E::mfma16(k1, q[2 * n + u], s1);
           }
         } else {
-          s0 = E::mfma16(t.k[0][n], q[n], s0);
-          s1 = E::mfma16(t.k[1][n], q[n], s1);
+          s0 = E::mfma16(kf[0][n], q[n], s0);
+          s1 = E::mfma16(kf[1][n], q[n], s1);
         }
       }
     }
@@ -250,10 +285,10 @@ struct Wave {
       s[i] = s0[i] * c2;
       s[4 + i] = s1[i] * c2;
     }
-    if (t.gone) {
+    if (t.live != ~0u) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const bool ok = voff[8 * j + e] >= 0;
+        const bool ok = t.live >> (8 * j + e) & 1;
         s[e] = ok ? s[e] : kNegInf;
 #pragma unroll
         for (int w = 0; w < T::VD; ++w) t.v[e][w] = ok ? t.v[e][w] : 0u;
@@ -344,13 +379,23 @@ __device__ __forceinline__ void store_out(uint8_t* o, const float (&x)[N]) {
   }
 }
 
-template <int D>
+struct Yes {
+  static constexpr bool value = true;
+};
+struct No {
+  static constexpr bool value = false;
+};
+
+template <typename E, int D>
 struct Shared {
   static constexpr int PAD = D + 4;  // float32 rows 4 banks apart
   union {
     struct {
-      int64_t k[kFill], v[kFill];
-    } off;
+      struct {
+        int64_t k[64], v[64];
+      } off[2];
+      u32x4 k[Tile<E, D>::STAGED ? kTile * Tile<E, D>::PR : 1];
+    } wave[kWaves];
     float o[kWaves][16][PAD];
   };
   float m[kWaves][16], l[kWaves][16];
@@ -359,11 +404,11 @@ struct Shared {
 template <typename E, int D>
 __global__ __launch_bounds__(kThreads) void paged_attn_kernel(const PagedAttnArgs a) {
   constexpr int NC = D / 16;
-  __shared__ Shared<D> sh;
+  __shared__ Shared<E, D> sh;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 15, j = lane >> 4;
-  const int streams = a.c.Hkv * a.row_tiles;
-  const int stream = blockIdx.x % streams, part = blockIdx.x / streams;
+  const int parts = a.parts ? a.parts : a.c.B;
+  const int stream = blockIdx.x / parts, part = blockIdx.x % parts;
   const int hkv = stream / a.row_tiles, h0 = stream % a.row_tiles * 16;  // first head of the tile within the group
   const int heads = imin(16, a.G - h0);
   const uint8_t* kb = a.c.k + int64_t(hkv) * a.c.sk[1];
@@ -371,6 +416,7 @@ __global__ __launch_bounds__(kThreads) void paged_attn_kernel(const PagedAttnArg
 
   int b, start, u, end;  // the run's sequence, its first unit, the run's units [u, end)
   int per = 0;
+  bool once = false;
   if (a.parts == 0) {
     b = part;
     start = u = 0;
@@ -379,6 +425,7 @@ __global__ __launch_bounds__(kThreads) void paged_attn_kernel(const PagedAttnArg
     int none, total;
     units_before(a, 0, none, total);
     per = units_per_part(total, a.parts, a.least);
+    once = total > a.keep_units;
     if (int64_t(part) * per >= total) return;
     u = part * per;
     end = imin(total, u + per);
@@ -399,39 +446,55 @@ __global__ __launch_bounds__(kThreads) void paged_attn_kernel(const PagedAttnArg
     w.load_q(a.q + int64_t(b) * a.sq[0] + int64_t(r < heads ? head : hkv * a.G) * a.sq[1], r < heads);
     w.reset();
     const int* table = a.c.table + int64_t(b) * a.c.table_stride;
-    for (int f0 = v0; f0 < v1; f0 += kFill) {
-      const int fill = imin(kFill, v1 - f0), tiles = (fill + kTile - 1) / kTile;
-      for (int i = tid; i < tiles * kTile; i += kThreads) {
-        int64_t ko = -1, vo = -1;
-        if (i < fill) {
-          const int key = visible_key(vis, f0 + i), pi = page_of(a.c.div, key);
-          const int page = table[pi], slot = key - pi * a.c.page_size;
-          if (page >= 0 && page < a.c.pages) {
-            ko = int64_t(page) * a.c.sk[0] + int64_t(slot) * a.c.sk[2];
-            vo = int64_t(page) * a.c.sv[0] + int64_t(slot) * a.c.sv[2];
-          }
-        }
-        sh.off.k[i] = ko;
-        sh.off.v[i] = vo;
+    // The wave's tiles, in pairs: tiles wave + 8p and wave + 8p + 4 of the run.  A lane works out the place of one of a
+    // pair's 64 keys: its page is asked for two pairs ahead, its offsets are in LDS one pair ahead.
+    const int n = v1 - v0, tiles = (n + kTile - 1) / kTile, mine = (tiles - wave + kWaves - 1) / kWaves, pairs = (mine + 1) / 2;
+    auto ask = [&](int p, int& slot) {
+      const int v = (wave + kWaves * (2 * p + (lane >> 5))) * kTile + (lane & 31);
+      slot = 0;
+      if (v >= n) return -1;
+      const int key = visible_key(vis, v0 + v), pi = page_of(a.c.div, key);
+      slot = key - pi * a.c.page_size;
+      return table[pi];
+    };
+    // (bit l: the key of lane l is on a page)
+    auto place = [&](int p, int page, int slot) -> unsigned long long {
+      const bool ok = page >= 0 && page < a.c.pages;
+      if (!ok) page = slot = 0;
+      sh.wave[wave].off[p & 1].k[lane] = int64_t(page) * a.c.sk[0] + int64_t(slot) * a.c.sk[2];
+      sh.wave[wave].off[p & 1].v[lane] = int64_t(page) * a.c.sv[0] + int64_t(slot) * a.c.sv[2];
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (the wave's other lanes read them)
+      return __ballot(ok);
+    };
+    auto logits = [&](int i) -> float* {  // of the wave's i-th tile
+      if (!a.sums || r >= heads) return nullptr;
+      const int at = v0 + (wave + kWaves * i) * kTile;
+      return a.logits + (((int64_t(hkv) * a.c.B + b) * a.max_units + at / kPagedUnit) * a.G + h0 + r) * kPagedUnit + at % kPagedUnit +
+             8 * j;
+    };
+    auto walk = [&](auto mode) {
+      constexpr bool ONCE = decltype(mode)::value;
+      auto& off = sh.wave[wave].off;
+      int slot, page = ask(0, slot);
+      unsigned long long live = place(0, page, slot);
+      page = ask(1, slot);
+      Tile<E, D> t, next;
+      w.template load<ONCE>(t, kb, vb, off[0].k, off[0].v, uint32_t(live));
+      for (int p = 0; p < pairs; ++p) {
+        const bool two = 2 * p + 1 < mine;
+        if (two) w.template load<ONCE>(next, kb, vb, off[p & 1].k + kTile, off[p & 1].v + kTile, uint32_t(live >> 32));
+        live = place(p + 1, page, slot);
+        page = ask(p + 2, slot);
+        w.step(t, a.c2, sh.wave[wave].k, logits(2 * p));
+        if (p + 1 < pairs) w.template load<ONCE>(t, kb, vb, off[(p + 1) & 1].k, off[(p + 1) & 1].v, uint32_t(live));
+        if (two) w.step(next, a.c2, sh.wave[wave].k, logits(2 * p + 1));
       }
-      __syncthreads();
-      Tile<E, D> t;
-      if (wave < tiles) w.load(t, kb, vb, sh.off.k + kTile * wave, sh.off.v + kTile * wave);
-      for (int i = wave; i < tiles; i += kWaves) {
-        Tile<E, D> next;
-        const int n = i + kWaves;
-        if (n < tiles) w.load(next, kb, vb, sh.off.k + kTile * n, sh.off.v + kTile * n);
-        float* logits = nullptr;
-        if (a.sums && r < heads) {
-          const int at = f0 + kTile * i;
-          logits = a.logits + (((int64_t(hkv) * a.c.B + b) * a.max_units + at / kPagedUnit) * a.G + h0 + r) * kPagedUnit +
-                   at % kPagedUnit + 8 * j;
-        }
-        w.step(t, a.c2, sh.off.v + kTile * i, logits);
-        if (n < tiles) t = next;
-      }
-      __syncthreads();
+    };
+    if (pairs > 0) {
+      if (once) walk(Yes{});
+      else walk(No{});
     }
+    __syncthreads();
 
     // the four waves' results, in wave order
     const float l = quarters_sum(w.l);
@@ -492,86 +555,145 @@ __global__ __launch_bounds__(kThreads) void paged_attn_kernel(const PagedAttnArg
   }
 }
 
-// A query head of a sequence that was cut: its pieces' results, added in order.  64 threads.
-template <typename E, int D>
-__global__ __launch_bounds__(64) void paged_join_kernel(const PagedAttnArgs a) {
-  const int hq = blockIdx.x % a.Hq, b = blockIdx.x / a.Hq;
-  int start, total;
-  units_before(a, b, start, total);
-  const int per = units_per_part(total, a.parts, a.least);
-  const int units = units_of(a, b), first = start / per, last = imin(a.parts - 1, (start + units - 1) / per);
-  if (first >= last) return;
-  const int hkv = hq / a.G, h = hq % a.G, stream = hkv * a.row_tiles + h / 16, oh = h % 16;
-  const int64_t base = int64_t(stream) * a.parts * 2;
-  const int lane = threadIdx.x;
-  float m = kNegInf;
-  for (int p = first + lane; p <= last; p += 64) m = fmaxf(m, a.part_ml[(base + part_slot(p, per, start)) * 32 + oh]);
-#pragma unroll
-  for (int x = 32; x >= 1; x >>= 1) m = fmaxf(m, __shfl_xor(m, x));
-  float top = m;
-  const float sink = a.sinks ? a.sinks[hq] * kLog2e : kNegInf;
-  top = fmaxf(top, sink);
-  const float ref = top == kNegInf ? 0.f : top;
-  constexpr int ND = (D + 63) / 64;
-  float sum = 0.f, o[ND] = {};
-  for (int p = first; p <= last; ++p) {
-    const int64_t slot = base + part_slot(p, per, start);
-    const float f = fast_exp2(a.part_ml[slot * 32 + oh] - ref);
-    sum += f * a.part_ml[slot * 32 + 16 + oh];
-    if (f != 0.f) {
-#pragma unroll
-      for (int i = 0; i < ND; ++i)
-        if (lane + 64 * i < D) o[i] += f * a.part_o[(slot * 16 + oh) * D + lane + 64 * i];
-    }
-  }
-  const float ls = sum + (sink == kNegInf ? 0.f : fast_exp2(sink - ref));
-  const float inv = sum == 0.f ? 0.f : a.oscale / ls;
-  uint8_t* out = a.o + int64_t(b) * a.so[0] + int64_t(hq) * a.so[1];
-#pragma unroll
-  for (int i = 0; i < ND; ++i)
-    if (lane + 64 * i < D) {
-      const float x[1] = {sum == 0.f ? 0.f : o[i] * inv};
-      store_out<E, 1>(out + (lane + 64 * i) * E::EB, x);
-    }
-  if (a.sums && lane == 0) a.lse[int64_t(b) * a.Hq + hq] = ref + fast_log2(ls);
+// ---- the second launch ---------------------------------------------------------------------------
+// Pieces of sequence b: those of the parts [first, last].
+struct Pieces {
+  int first, last, start, per;
+};
+__device__ __forceinline__ Pieces pieces_of(const PagedAttnArgs& a, int b) {
+  Pieces p{0, 0, 0, 0};
+  if (a.parts == 0) return p;
+  int total;
+  units_before(a, b, p.start, total);
+  p.per = units_per_part(total, a.parts, a.least);
+  p.first = p.start / p.per;
+  p.last = imin(a.parts - 1, (p.start + units_of(a, b) - 1) / p.per);
+  return p;
 }
 
-// sums[b, hkv, key] += sum over the group's heads of 2^(logit - lse), a thread a key: no order to choose, no atomics.
-constexpr int kSumKeys = 1024;
-__global__ __launch_bounds__(kThreads) void paged_sums_kernel(const PagedAttnArgs a) {
-  const int chunks = (a.max_units * kPagedUnit + kSumKeys - 1) / kSumKeys;
-  const int chunk = blockIdx.x % chunks, stream = blockIdx.x / chunks, hkv = stream % a.c.Hkv, b = stream / a.c.Hkv;
-  const Visible vis = visible(seq_len(a.c, b), a.W, a.S);
-  const int end = imin(vis.count, (chunk + 1) * kSumKeys);
-  for (int v = chunk * kSumKeys + threadIdx.x; v < end; v += kThreads) {
-    const float* x = a.logits + ((int64_t(hkv) * a.c.B + b) * a.max_units + v / kPagedUnit) * a.G * kPagedUnit + v % kPagedUnit;
-    const float* lse = a.lse + int64_t(b) * a.Hq + hkv * a.G;
-    float w = 0.f;
-    for (int g = 0; g < a.G; ++g) {
-      const float s = x[g * kPagedUnit];
-      w += s == kNegInf ? 0.f : fast_exp2(s - lse[g]);
-    }
-    a.sums[int64_t(b) * a.ssum[0] + int64_t(hkv) * a.ssum[1] + visible_key(vis, v)] += w;
+// Query head hq of sequence b, if it was cut: its pieces' results.  D / 4 threads take a piece; every thread adds its
+// pieces in order, then the groups of threads are added in order.
+template <typename E, int D>
+__device__ __forceinline__ void join_head(const PagedAttnArgs& a, int b, int hq, float* smem) {
+  constexpr int T = D / 4, GROUPS = kThreads / T;
+  const Pieces ps = pieces_of(a, b);
+  if (ps.first >= ps.last) return;
+  const int hkv = hq / a.G, h = hq % a.G, oh = h % 16;
+  const int64_t base = int64_t(hkv * a.row_tiles + h / 16) * a.parts * 2;
+  const int tid = threadIdx.x, lane = tid & 63, group = tid / T, d = tid % T * 4;
+  float m = kNegInf;
+  for (int p = ps.first + lane; p <= ps.last; p += 64) m = fmaxf(m, a.part_ml[(base + part_slot(p, ps.per, ps.start)) * 32 + oh]);
+#pragma unroll
+  for (int x = 32; x >= 1; x >>= 1) m = fmaxf(m, __shfl_xor(m, x));
+  const float sink = a.sinks ? a.sinks[hq] * kLog2e : kNegInf, top = fmaxf(m, sink), ref = top == kNegInf ? 0.f : top;
+  float sum = 0.f;
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int p = ps.first + group; p <= ps.last; p += GROUPS) {
+    const int64_t slot = base + part_slot(p, ps.per, ps.start);
+    const float f = fast_exp2(a.part_ml[slot * 32 + oh] - ref);
+    const f32x4 x = *reinterpret_cast<const f32x4*>(a.part_o + (slot * 16 + oh) * D + d);
+    sum += f * a.part_ml[slot * 32 + 16 + oh];
+    o += f * x;
   }
+  // [group][D], [group] sums
+#pragma unroll
+  for (int i = 0; i < 4; ++i) smem[group * D + d + i] = o[i];
+  if (d == 0) smem[GROUPS * D + group] = sum;
+  __syncthreads();
+  if (tid < D) {
+    float x = 0.f, s = 0.f;
+#pragma unroll 8
+    for (int g = 0; g < GROUPS; ++g) {
+      x += smem[g * D + tid];
+      s += smem[GROUPS * D + g];
+    }
+    const float ls = s + (sink == kNegInf ? 0.f : fast_exp2(sink - ref));
+    const float out[1] = {s == 0.f ? 0.f : x * (a.oscale / ls)};
+    store_out<E, 1>(a.o + int64_t(b) * a.so[0] + int64_t(hq) * a.so[1] + tid * E::EB, out);
+  }
+}
+
+// sums[b, hkv, key] += sum over the group's heads of 2^(logit - lse): a thread takes keys, so there is no order to choose and
+// no atomic.
+constexpr int kSumKeys = 1024;
+constexpr int kSumHeads = 64;  // heads whose lse a workgroup holds at a time
+__device__ __forceinline__ void add_weights(const PagedAttnArgs& a, int b, int hkv, int chunk, float* smem) {
+  const Visible vis = visible(seq_len(a.c, b), a.W, a.S);
+  const int v0 = chunk * kSumKeys + 4 * int(threadIdx.x);
+  if (chunk * kSumKeys >= vis.count) return;
+  const Pieces ps = pieces_of(a, b);
+  float w[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int g0 = 0; g0 < a.G; g0 += kSumHeads) {
+    const int ng = imin(kSumHeads, a.G - g0);
+    if (g0) __syncthreads();
+    // four threads work out a head's lse
+    const int g = g0 + int(threadIdx.x) / 4, sub = threadIdx.x & 3;
+    if (g < a.G) {
+      const int hq = hkv * a.G + g;
+      float lse;
+      if (ps.first >= ps.last) {
+        lse = a.lse[int64_t(b) * a.Hq + hq];
+      } else {
+        const float* ml = a.part_ml + int64_t(hkv * a.row_tiles + g / 16) * a.parts * 2 * 32 + g % 16;
+        float m = a.sinks ? a.sinks[hq] * kLog2e : kNegInf;
+        const float sink = m;
+        for (int p = ps.first + sub; p <= ps.last; p += 4) m = fmaxf(m, ml[part_slot(p, ps.per, ps.start) * 32]);
+        m = fmaxf(m, __shfl_xor(m, 1));
+        m = fmaxf(m, __shfl_xor(m, 2));
+        const float ref = m == kNegInf ? 0.f : m;
+        float s = sub == 0 && sink != kNegInf ? fast_exp2(sink - ref) : 0.f;
+        for (int p = ps.first + sub; p <= ps.last; p += 4) {
+          const int slot = part_slot(p, ps.per, ps.start) * 32;
+          s += fast_exp2(ml[slot] - ref) * ml[slot + 16];
+        }
+        s += __shfl_xor(s, 1);
+        s += __shfl_xor(s, 2);
+        lse = ref + fast_log2(s);
+      }
+      if (sub == 0) smem[g - g0] = lse;
+    }
+    __syncthreads();
+    if (v0 < vis.count) {
+      const float* x = a.logits +
+                       ((int64_t(hkv) * a.c.B + b) * a.max_units + v0 / kPagedUnit) * a.G * kPagedUnit + g0 * kPagedUnit + v0 % kPagedUnit;
+#pragma unroll 8
+      for (int i = 0; i < ng; ++i) {
+        const f32x4 s = *reinterpret_cast<const f32x4*>(x + i * kPagedUnit);
+        const float lse = smem[i];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) w[c] += s[c] == kNegInf ? 0.f : fast_exp2(s[c] - lse);
+      }
+    }
+  }
+  float* out = a.sums + int64_t(b) * a.ssum[0] + int64_t(hkv) * a.ssum[1];
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+    if (v0 + c < vis.count) out[visible_key(vis, v0 + c)] += w[c];
+}
+
+// Workgroups [0, joins) join heads, the ones behind them add weights.
+template <typename E, int D>
+__global__ __launch_bounds__(kThreads) void paged_finish_kernel(const PagedAttnArgs a, unsigned joins) {
+  __shared__ float smem[kThreads * 4 + 64];
+  if (blockIdx.x < joins) {
+    join_head<E, D>(a, blockIdx.x / a.Hq, blockIdx.x % a.Hq, smem);
+    return;
+  }
+  const unsigned i = blockIdx.x - joins, chunks = unsigned((a.max_units * kPagedUnit + kSumKeys - 1) / kSumKeys);
+  add_weights(a, int(i / chunks / unsigned(a.c.Hkv)), int(i / chunks % unsigned(a.c.Hkv)), int(i % chunks), smem);
 }
 
 template <typename E, int D>
 hipError_t run(const PagedAttnArgs& a, hipStream_t s) {
-  const int streams = a.c.Hkv * a.row_tiles;
-  hipLaunchKernelGGL((paged_attn_kernel<E, D>), dim3(unsigned(streams) * unsigned(a.parts ? a.parts : a.c.B)), dim3(kThreads), 0, s, a);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return e;
-  if (a.parts) {
-    hipLaunchKernelGGL((paged_join_kernel<E, D>), dim3(unsigned(a.Hq) * unsigned(a.c.B)), dim3(64), 0, s, a);
-    e = hipGetLastError();
-    if (e != hipSuccess) return e;
-  }
-  if (a.sums) {
-    const unsigned chunks = unsigned((a.max_units * kPagedUnit + kSumKeys - 1) / kSumKeys);
-    hipLaunchKernelGGL(paged_sums_kernel, dim3(chunks * unsigned(a.c.Hkv) * unsigned(a.c.B)), dim3(kThreads), 0, s, a);
-    e = hipGetLastError();
-  }
-  return e;
+  const unsigned streams = unsigned(a.c.Hkv * a.row_tiles), B = unsigned(a.c.B);
+  hipLaunchKernelGGL((paged_attn_kernel<E, D>), dim3(streams * (a.parts ? unsigned(a.parts) : B)), dim3(kThreads), 0, s, a);
+  const hipError_t e = hipGetLastError();
+  const unsigned joins = a.parts ? unsigned(a.Hq) * B : 0u;
+  const unsigned adds = a.sums ? unsigned((a.max_units * kPagedUnit + kSumKeys - 1) / kSumKeys) * unsigned(a.c.Hkv) * B : 0u;
+  if (e != hipSuccess || joins + adds == 0) return e;
+  hipLaunchKernelGGL((paged_finish_kernel<E, D>), dim3(joins + adds), dim3(kThreads), 0, s, a, joins);
+  return hipGetLastError();
 }
 
 template <typename E>
