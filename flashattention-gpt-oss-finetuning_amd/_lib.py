@@ -243,7 +243,7 @@ def lib() -> ctypes.CDLL:
             L.fa_paged_workspace_bytes.restype = ctypes.c_size_t
             L.fa_paged_attention.argtypes = [ctypes.POINTER(PagedAttentionParams), ctypes.c_void_p, ctypes.c_size_t,
                                              ctypes.c_void_p]
-            L.fa_paged_evict_workspace_bytes.argtypes = [ctypes.c_int32] * 3
+            L.fa_paged_evict_workspace_bytes.argtypes = [ctypes.c_int32] * 4
             L.fa_paged_evict_workspace_bytes.restype = ctypes.c_size_t
             L.fa_paged_evict.argtypes = [ctypes.POINTER(PagedEvictParams), ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
             L.fa_check_fwd.argtypes = [ctypes.POINTER(FwdParams)]

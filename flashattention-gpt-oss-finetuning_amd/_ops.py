@@ -651,7 +651,8 @@ def paged_evict(k_pages, v_pages, block_table, lens, weight_sums, keep: int, new
     p.new_table_width = _fits_i32(new_table.shape[1], "the new_table's width")
     p.new_lens = new_lens.data_ptr()
     p.keep, p.sink, p.recent = _fits_i32(keep, "keep"), _fits_i32(sink, "sink_size"), _fits_i32(recent, "recent")
-    nbytes = int(_lib.lib().fa_paged_evict_workspace_bytes(B, Hkv, p.keep))
+    tokens = _i32(p.cache.table_width * p.cache.page_size)
+    nbytes = int(_lib.lib().fa_paged_evict_workspace_bytes(B, Hkv, p.keep, tokens))
     ws = torch.empty((max(nbytes, 256),), dtype=torch.uint8, device=lens.device)
     _run_paged("fa_paged_evict", lens.device, ctypes.byref(p), ctypes.c_void_p(ws.data_ptr()), ctypes.c_size_t(ws.numel()))
     _changed(k_pages, v_pages)

@@ -126,6 +126,26 @@ int plan(const fa_paged_attention_params* p, Plan* r) {
   return FA_OK;
 }
 
+// Weights that a thread of the selection holds where one workgroup a (sequence, KV head) does not hold them all.
+constexpr int kSplitEach = 8;
+
+// An eviction's launches and the bytes of its workspace.
+struct EvictRoom {
+  int each, chunks;
+  size_t kept, state, counts;
+};
+EvictRoom evict_room(int64_t heads, int32_t keep, int64_t tokens) {
+  EvictRoom r{};
+  r.each = tokens <= 4096 ? 4 : tokens <= 8192 ? 8 : tokens <= 16384 ? 16 : kSplitEach;
+  r.chunks = int((tokens + 1024 * r.each - 1) / (1024 * r.each));
+  r.kept = align256(size_t(heads) * keep * sizeof(int32_t));
+  if (r.chunks > 1) {
+    r.state = align256(size_t(heads) * r.chunks * 3 * sizeof(int32_t));
+    r.counts = align256(size_t(heads) * r.chunks * 3 * 2048 * sizeof(uint16_t));
+  }
+  return r;
+}
+
 }  // namespace
 
 extern "C" {
@@ -206,9 +226,10 @@ int fa_paged_attention(const fa_paged_attention_params* p, void* workspace, size
   return status(fa::launch_paged_attention(a, p->dtype, c.dtype, c.head_dim, static_cast<hipStream_t>(stream)));
 }
 
-size_t fa_paged_evict_workspace_bytes(int32_t batch, int32_t heads_kv, int32_t keep) {
-  if (batch < 1 || heads_kv < 1 || keep < 1) return 0;
-  return align256(size_t(batch) * heads_kv * keep * sizeof(int32_t));
+size_t fa_paged_evict_workspace_bytes(int32_t batch, int32_t heads_kv, int32_t keep, int32_t tokens) {
+  if (batch < 1 || heads_kv < 1 || keep < 1 || tokens < 1) return 0;
+  const EvictRoom r = evict_room(int64_t(batch) * heads_kv, keep, tokens);
+  return r.kept + r.state + r.counts;
 }
 
 int fa_paged_evict(const fa_paged_evict_params* p, void* workspace, size_t workspace_bytes, void* stream) {
@@ -227,12 +248,13 @@ int fa_paged_evict(const fa_paged_evict_params* p, void* workspace, size_t works
     return FA_ERR_ALIGN;
   for (int i = 0; i < 2; ++i)
     if (p->sums_stride[i] < 0 || p->new_sums_stride[i] < 0) return FA_ERR_ALIGN;
-  if (!workspace || !aligned(workspace, 256) || workspace_bytes < fa_paged_evict_workspace_bytes(c.batch, c.heads_kv, p->keep))
+  if (!workspace || !aligned(workspace, 256) || workspace_bytes < fa_paged_evict_workspace_bytes(c.batch, c.heads_kv, p->keep, int32_t(tokens)))
     return FA_ERR_WORKSPACE;
   const int row = c.head_dim * elem_bytes(c.dtype);
-  // workgroups of the two launches: 1024 threads a (sequence, KV head), and 1024 pieces of 16 bytes of kept entries
+  // workgroups of the launches: 1024 threads a chunk, and one for 1024 pieces of 16 bytes of kept entries
   const int64_t heads = int64_t(c.batch) * c.heads_kv, chunk = 1024 / (row / 16);
-  if (!fa::grid_fits(heads, 1024) || !fa::grid_fits(heads * ((p->keep + chunk - 1) / chunk))) return FA_ERR_OVERFLOW;
+  const EvictRoom room = evict_room(heads, p->keep, tokens);
+  if (!fa::grid_fits(heads * room.chunks, 1024) || !fa::grid_fits(heads * ((p->keep + chunk - 1) / chunk))) return FA_ERR_OVERFLOW;
   fa::EvictArgs a{};
   a.c = cache_args(c);
   a.sums = p->sums;
@@ -248,7 +270,12 @@ int fa_paged_evict(const fa_paged_evict_params* p, void* workspace, size_t works
   a.keep = p->keep;
   a.S = p->sink;
   a.R = p->recent;
-  a.kept = static_cast<int*>(workspace);
+  a.each = room.each;
+  a.chunks = room.chunks;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  a.kept = reinterpret_cast<int*>(ws);
+  a.state = reinterpret_cast<int*>(ws + room.kept);
+  a.counts = reinterpret_cast<uint16_t*>(ws + room.kept + room.state);
   return status(fa::launch_paged_evict(a, row, static_cast<hipStream_t>(stream)));
 }
 

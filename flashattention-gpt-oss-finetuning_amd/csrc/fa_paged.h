@@ -64,7 +64,11 @@ struct EvictArgs {
   int64_t new_table_stride;
   int* new_lens;
   int keep, S, R;
-  int* kept;              // workspace: [B][Hkv][keep] entries kept, in order
+  int each, chunks;       // chunks of 1024 each entries, a (sequence, KV head); each is 4, 8 or 16
+  // workspace
+  int* kept;              // [B][Hkv][keep] entries kept, in order
+  int* state;             // with several chunks: [B][Hkv][chunks][3]
+  uint16_t* counts;       // with several chunks: [B][Hkv][3 digits][chunks][2048]
 };
 
 // dtype and cache are fa_dtype values

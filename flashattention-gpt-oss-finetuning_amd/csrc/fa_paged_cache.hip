@@ -7,8 +7,8 @@
 //
 // paged_select_kernel.  Of a (sequence, KV head)'s n entries the first S and the last R stay, and of the others the
 // keep - S - R of the largest weight, the lower index first among equals (NaN counts as the largest).  The weights are
-// mapped to unsigned numbers of the same order; four passes of 8 bits find the smallest one that stays, T, and how
-// many equal to T do; a last pass in index order numbers the entries that stay.
+// mapped to unsigned numbers of the same order; three digits of them, from the top, find the smallest one that stays and
+// how many equal to it do; then the entries that stay are numbered in order.
 // paged_gather_kernel.  Entry r of those kept goes to position r on the pages of the new table.  Those are other pages
 // than the old ones, so no entry is read after it is overwritten and all are copied at once.
 #include <hip/hip_runtime.h>
@@ -124,102 +124,224 @@ __device__ __forceinline__ uint32_t order_of(float x) {
   return u >> 31 ? ~u : u | 0x80000000u;
 }
 
-__global__ __launch_bounds__(kSelectThreads) void paged_select_kernel(const EvictArgs a) {
-  const int hkv = blockIdx.x % a.c.Hkv, b = blockIdx.x / a.c.Hkv;
+// Digits of those numbers, from the top: 11, 11 and 10 bits.
+constexpr int kDigits = 3, kBins = 2048;
+__device__ __forceinline__ uint32_t digit_of(uint32_t u, int q) { return q == 0 ? u >> 21 : q == 1 ? u >> 10 & 2047 : u & 1023; }
+__device__ __forceinline__ uint32_t digits_above(uint32_t u, int q) { return q == 0 ? 0u : q == 1 ? u >> 21 : u >> 10; }
+__device__ __forceinline__ uint32_t with_digit(uint32_t prefix, uint32_t d, int q) { return prefix << (q == 2 ? 10 : 11) | d; }
+
+constexpr int kSelectWaves = kSelectThreads / 64;
+
+constexpr int kSelectMost = 16;  // entries that a thread has in registers, at most
+
+// A chunk's entries in registers: entry first + 1024 e + tid is x[e], u[e] its place in the order.
+template <int EACH>
+struct Entries {
+  float x[EACH];
+  uint32_t u[EACH];
+  uint32_t open;  // bit e: the entry may be chosen; the others stay, or are none
+};
+
+struct SelectShared {
+  uint32_t hist[kBins];
+  int wave[2][kSelectWaves];
+  uint32_t runs[kSelectMost * kSelectWaves];
+  uint32_t digit;
+  int need, prior, equal;
+};
+
+template <int EACH>
+__device__ __forceinline__ void read_entries(Entries<EACH>& t, const float* x, int first, int n, int lo, int hi) {
+  const int tid = threadIdx.x;
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) {
+    const int i = first + e * kSelectThreads + tid;
+    t.x[e] = i < n ? x[i] : 0.f;
+  }
+  t.open = 0;
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) {
+    const int i = first + e * kSelectThreads + tid;
+    t.u[e] = order_of(t.x[e]);
+    t.open |= uint32_t(i >= lo && i < hi) << e;
+  }
+}
+
+// sh.hist: how many open entries whose digits above digit q are `prefix` have each value of that digit.
+template <int EACH>
+__device__ __forceinline__ void count_digits(SelectShared& sh, const Entries<EACH>& t, uint32_t prefix, int q) {
+  sh.hist[threadIdx.x] = sh.hist[threadIdx.x + kSelectThreads] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < EACH; ++e)
+    if ((t.open >> e & 1) && digits_above(t.u[e], q) == prefix) atomicAdd(&sh.hist[digit_of(t.u[e], q)], 1u);
+  __syncthreads();
+}
+
+// cnt: entries in this thread's bins 2047 - 2 tid and 2046 - 2 tid; old: those of earlier chunks.  Finds the bin of the
+// need-th entry from the largest: its digit; need becomes the number of its entries that stay; prior grows by the
+// entries of earlier chunks in larger bins; equal: theirs in this bin.
+__device__ __forceinline__ uint32_t find_digit(SelectShared& sh, const int (&cnt)[2], const int (&old)[2], int& need, int& prior, int& equal) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int n = seq_len(a.c, b), m = imin(n, a.keep);
-  const float* x = a.sums + int64_t(b) * a.ssum[0] + int64_t(hkv) * a.ssum[1];
+  const int both = cnt[0] + cnt[1], both_old = old[0] + old[1];
+  int x = both, y = both_old;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int p = __shfl_up(x, o), q = __shfl_up(y, o);
+    if (lane >= o) {
+      x += p;
+      y += q;
+    }
+  }
+  if (lane == 63) {
+    sh.wave[0][wave] = x;
+    sh.wave[1][wave] = y;
+  }
+  __syncthreads();
+  int before = x - both, before_old = y - both_old;
+#pragma unroll
+  for (int w = 0; w < kSelectWaves; ++w) {
+    before += w < wave ? sh.wave[0][w] : 0;
+    before_old += w < wave ? sh.wave[1][w] : 0;
+  }
+  if (before < need && before + both >= need) {  // (one thread: 1 <= need <= all entries)
+    const int i = before + cnt[0] >= need ? 0 : 1;
+    sh.digit = uint32_t(kBins - 1 - 2 * tid - i);
+    sh.need = need - before - (i ? cnt[0] : 0);
+    sh.prior = before_old + (i ? old[0] : 0);
+    sh.equal = i ? old[1] : old[0];
+  }
+  __syncthreads();
+  need = sh.need;
+  prior += sh.prior;
+  equal = sh.equal;
+  return sh.digit;
+}
+
+// Numbers the chunk's entries that stay, in order, and writes them: those that are not open, the open ones above `least`, and
+// of those equal to it the first `need` (equal of which are in earlier chunks).  rank: entries of earlier chunks that
+// stay for another reason.
+template <int EACH>
+__device__ __forceinline__ void write_kept(SelectShared& sh, const Entries<EACH>& t, int first, int n, int m, uint32_t least, int need, int rank, int equal,
+                                           int* kept, float* y) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const unsigned long long below = (1ull << lane) - 1;
+  uint32_t mine[EACH];  // entries of this wave's row e before this lane: those that stay, and << 16 the equal ones
+  uint32_t stays = 0, equals = 0;
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) {
+    const bool open = t.open >> e & 1, have = first + e * kSelectThreads + tid < n;
+    const bool s = have && (!open || t.u[e] > least), q = open && t.u[e] == least;
+    const unsigned long long ms = __ballot(s), mq = __ballot(q);
+    mine[e] = uint32_t(__popcll(ms & below)) | uint32_t(__popcll(mq & below)) << 16;
+    stays |= uint32_t(s) << e;
+    equals |= uint32_t(q) << e;
+    if (lane == 0) sh.runs[e * kSelectWaves + wave] = uint32_t(__popcll(ms)) | uint32_t(__popcll(mq)) << 16;
+  }
+  __syncthreads();
+  if (wave == 0) {  // exclusive sums over the runs, in order (both halves stay below 2^16: a chunk has 2^14 entries)
+    constexpr int PER = EACH * kSelectWaves / 64;  // (EACH is a multiple of 4)
+    uint32_t c[PER], all = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) all += c[i] = sh.runs[lane * PER + i];
+    uint32_t x = all;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const uint32_t p = uint32_t(__shfl_up(int(x), o));
+      if (lane >= o) x += p;
+    }
+    x -= all;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      sh.runs[lane * PER + i] = x;
+      x += c[i];
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) {
+    const uint32_t x = sh.runs[e * kSelectWaves + wave] + mine[e];
+    const int before = equal + int(x >> 16);  // equal entries before this one
+    if ((stays >> e & 1) || ((equals >> e & 1) && before < need)) {
+      const int r = rank + int(x & 0xffff) + imin(before, need);
+      if (unsigned(r) < unsigned(m)) {  // (always, unless the weights change under the running call)
+        kept[r] = first + e * kSelectThreads + tid;
+        y[r] = t.x[e];
+      }
+    }
+  }
+}
+
+// One chunk of 1024 EACH entries of a (sequence, KV head) a workgroup, in registers.  Where that is all of them (a.chunks = 1)
+// one launch does everything.  Otherwise launch `stage` = 0, 1, 2 leaves the chunks' counts of digit `stage` in the
+// workspace, from which every workgroup of the next launch finds the digit for itself, and launch 3 writes: no
+// atomic in memory, nothing to clear, and nobody waits for another workgroup.
+template <int EACH>
+__global__ __launch_bounds__(kSelectThreads) void paged_select_kernel(const EvictArgs a, int stage) {
+  constexpr int kChunk = EACH * kSelectThreads;
+  __shared__ SelectShared sh;
+  const int chunk = blockIdx.x % a.chunks, row = blockIdx.x / a.chunks, hkv = row % a.c.Hkv, b = row / a.c.Hkv;
+  const int tid = threadIdx.x;
+  const int n = seq_len(a.c, b), m = imin(n, a.keep), first = chunk * kChunk;
+  const bool last = a.chunks == 1 || stage == kDigits;
   float* y = a.new_sums + int64_t(b) * a.snew[0] + int64_t(hkv) * a.snew[1];
-  int* kept = a.kept + (int64_t(b) * a.c.Hkv + hkv) * a.keep;
-  if (hkv == 0 && tid == 0) a.new_lens[b] = m;
-  for (int i = m + tid; i < a.sums_width; i += kSelectThreads) y[i] = 0.f;
-  if (n <= a.keep) {
-    for (int i = tid; i < n; i += kSelectThreads) {
-      y[i] = x[i];
-      kept[i] = i;
-    }
-    return;
+  if (last) {
+    if (hkv == 0 && chunk == 0 && tid == 0) a.new_lens[b] = m;
+    const int end = chunk == a.chunks - 1 ? a.sums_width : imin(first + kChunk, a.sums_width);
+    for (int i = imax(m, first) + tid; i < end; i += kSelectThreads) y[i] = 0.f;
   }
-  __shared__ int hist[256];
-  __shared__ uint32_t s_prefix;
-  __shared__ int s_need;
-  __shared__ uint32_t s_wave[kSelectThreads / 64];
-  const int lo = a.S, hi = n - a.R;  // the entries to choose from; hi - lo > keep - S - R
-  if (tid == 0) {
-    s_prefix = 0;
-    s_need = a.keep - a.S - a.R;
-  }
-  // the bits of the smallest number that stays, from the top; `need` counts those still to be found among
-  // the numbers that share them
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    if (tid < 256) hist[tid] = 0;
-    __syncthreads();
-    const uint32_t prefix = s_prefix;
-    const int need = s_need;
-    for (int i = lo + tid; i < hi; i += kSelectThreads) {
-      const uint32_t u = order_of(x[i]);
-      if (shift == 24 || u >> (shift + 8) == prefix) atomicAdd(&hist[u >> shift & 255], 1);
+  // (entries to choose from: all but the first S and the last R, none where nothing is evicted or all stay by their place)
+  const int choose = n > a.keep ? a.keep - a.S - a.R : 0;
+  if (first >= n || (choose == 0 && !last)) return;
+  const int lo = n > a.keep ? a.S : 0, hi = n > a.keep ? n - a.R : 0;
+  Entries<EACH> t;
+  read_entries(t, a.sums + int64_t(b) * a.ssum[0] + int64_t(hkv) * a.ssum[1], first, n, lo, hi);
+  uint32_t prefix = choose > 0 ? 0u : 0xffffffffu;  // (nothing to choose: no number is above, and none equal is needed)
+  int need = choose, prior = 0, equal = 0;
+  if (choose > 0 && a.chunks == 1) {
+    for (int q = 0; q < kDigits; ++q) {
+      count_digits(sh, t, prefix, q);
+      const int cnt[2] = {int(sh.hist[kBins - 1 - 2 * tid]), int(sh.hist[kBins - 2 - 2 * tid])}, old[2] = {0, 0};
+      prefix = with_digit(prefix, find_digit(sh, cnt, old, need, prior, equal), q);
     }
-    __syncthreads();
-    if (wave == 0) {
-      // digits from 255 down: lane l has digits 255 - 4l .. 252 - 4l
-      int c[4], t = 0;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) t += c[i] = hist[255 - 4 * lane - i];
-      int before = t;
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const int z = __shfl_up(before, o);
-        if (lane >= o) before += z;
+  } else if (choose > 0) {
+    const int chunks = (n + kChunk - 1) / kChunk;
+    int* state = a.state + (int64_t(row) * a.chunks + chunk) * 3;  // this workgroup's prefix, need and prior
+    uint16_t* counts = a.counts + int64_t(row) * kDigits * a.chunks * kBins;  // [digit][chunk][2047 - value]
+    if (stage > 0) {
+      if (stage > 1) {
+        prefix = uint32_t(state[0]);
+        need = state[1];
+        prior = state[2];
       }
-      before -= t;  // numbers of larger digits than this lane's
-      // (need = 0: no number stays; T is then above all of them)
-      if (need > 0 && before < need && before + t >= need) {
-        int i = 0;
-        while (before + c[i] < need) before += c[i++];
-        s_prefix = prefix << 8 | uint32_t(255 - 4 * lane - i);
-        s_need = need - before;
+      const uint32_t* of = reinterpret_cast<const uint32_t*>(counts + int64_t(stage - 1) * a.chunks * kBins) + tid;
+      int cnt[2] = {0, 0}, old[2] = {0, 0};
+#pragma unroll 8
+      for (int c = 0; c < chunks; ++c) {
+        const uint32_t x = of[c * (kBins / 2)];
+        if (c == chunk) {
+          old[0] = cnt[0];
+          old[1] = cnt[1];
+        }
+        cnt[0] += int(x & 0xffff);
+        cnt[1] += int(x >> 16);
+      }
+      prefix = with_digit(prefix, find_digit(sh, cnt, old, need, prior, equal), stage - 1);
+      if (!last && tid == 0) {
+        state[0] = int(prefix);
+        state[1] = need;
+        state[2] = prior;
       }
     }
-    __syncthreads();
+    if (!last) {
+      count_digits(sh, t, prefix, stage);
+      reinterpret_cast<uint32_t*>(counts + (int64_t(stage) * a.chunks + chunk) * kBins)[tid] =
+          sh.hist[kBins - 1 - 2 * tid] | sh.hist[kBins - 2 - 2 * tid] << 16;
+      return;
+    }
   }
-  const uint32_t T = s_prefix;
-  const int need = s_need;
-  const bool none = a.keep == a.S + a.R;
-  int above = 0, equal = 0;  // entries before the tile that stay for good, and equal ones
-  for (int i0 = 0; i0 < n; i0 += kSelectThreads) {
-    const int i = i0 + tid;
-    bool stays = false, eq = false;
-    float w = 0.f;
-    if (i < n) {
-      w = x[i];
-      const uint32_t u = order_of(w);
-      stays = i < lo || i >= hi || (!none && u > T);
-      eq = !stays && !none && u == T;
-    }
-    const unsigned long long ms = __ballot(stays), me = __ballot(eq);
-    if (lane == 0) s_wave[wave] = uint32_t(__popcll(ms)) | uint32_t(__popcll(me)) << 16;
-    __syncthreads();
-    uint32_t before = 0, all = 0;
-#pragma unroll
-    for (int v = 0; v < kSelectThreads / 64; ++v) {
-      const uint32_t c = s_wave[v];
-      before += v < wave ? c : 0u;
-      all += c;
-    }
-    const unsigned long long below = (1ull << lane) - 1;
-    const int sb = above + int(before & 0xffff) + __popcll(ms & below), eb = equal + int(before >> 16) + __popcll(me & below);
-    if (stays || (eq && eb < need)) {
-      const int r = sb + imin(eb, need);
-      if (r < m) {  // (always, unless the weights change under the running call)
-        kept[r] = i;
-        y[r] = w;
-      }
-    }
-    above += int(all & 0xffff);
-    equal += int(all >> 16);
-    __syncthreads();
-  }
+  const int fixed = n > a.keep ? imin(first, lo) + imax(0, first - hi) : first;  // entries of earlier chunks that stay by their place
+  write_kept(sh, t, first, n, m, prefix, need, fixed + prior, equal, a.kept + int64_t(row) * a.keep, y);
 }
 
 // Entries of a workgroup: kThreads / pieces a round.
@@ -274,9 +396,14 @@ hipError_t launch_paged_append(const AppendArgs& a, int dtype, int cache, int D,
 }
 
 hipError_t launch_paged_evict(const EvictArgs& a, int row_bytes, hipStream_t s) {
-  hipLaunchKernelGGL(paged_select_kernel, dim3(unsigned(a.c.B * a.c.Hkv)), dim3(kSelectThreads), 0, s, a);
-  const hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return e;
+  for (int stage = a.chunks == 1 ? kDigits : 0; stage <= kDigits; ++stage) {
+    const dim3 grid(unsigned(a.chunks) * unsigned(a.c.B * a.c.Hkv)), block(kSelectThreads);
+    if (a.each == 4) hipLaunchKernelGGL(paged_select_kernel<4>, grid, block, 0, s, a, stage);
+    else if (a.each == 8) hipLaunchKernelGGL(paged_select_kernel<8>, grid, block, 0, s, a, stage);
+    else hipLaunchKernelGGL(paged_select_kernel<16>, grid, block, 0, s, a, stage);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
   switch (row_bytes / 16) {
     case 2: return gather<2>(a, s);
     case 4: return gather<4>(a, s);

@@ -322,7 +322,7 @@ int fa_paged_attention(const fa_paged_attention_params* p, void* workspace, size
  * positions 0, 1, ... of the pages of new_table ([batch][new_table_width]), which must not be pages that the call reads;
  * shorter sequences are copied whole.  new_sums gets the kept entries' sums and zeros behind them, new_lens
  * min(n, keep).  Positions have no meaning for the window or the sinks of an attention call any more.  The
- * workspace holds at least fa_paged_evict_workspace_bytes(batch, heads_kv, keep). */
+ * workspace holds at least fa_paged_evict_workspace_bytes(), whose `tokens` are the table's: table_width * page_size. */
 typedef struct fa_paged_evict_params {
   fa_paged_cache cache;
   const float* sums;      /* [batch, Hkv, sums_width] */
@@ -334,7 +334,7 @@ typedef struct fa_paged_evict_params {
   int32_t* new_lens;      /* [batch] */
   int32_t sums_width, new_table_width, keep, sink, recent;
 } fa_paged_evict_params;
-size_t fa_paged_evict_workspace_bytes(int32_t batch, int32_t heads_kv, int32_t keep);
+size_t fa_paged_evict_workspace_bytes(int32_t batch, int32_t heads_kv, int32_t keep, int32_t tokens);
 int fa_paged_evict(const fa_paged_evict_params* p, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Host-only argument checks used by fa_fwd / fa_bwd (no HIP call is made). */

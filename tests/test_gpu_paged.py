@@ -278,6 +278,10 @@ EVICT = [
     ("fp8", 64, 2, 16, "hnd", (100, 33), 1, 0, 0),
     ("fp8", 128, 2, 24, "nhd", (1100, 33), 100, 1, 1),
     ("fp32", 16, 1, 16, "hnd", (100, 33), 50, 10, 40),
+    # more entries than a workgroup of the selection holds
+    ("fp16", 16, 2, 64, "nhd", (40000, 16385, 5, 20000, 16384), 3000, 4, 100),
+    ("bf16", 16, 1, 16, "hnd", (40001, 33000), 20000, 17000, 0),
+    ("bf16", 16, 1, 16, "hnd", (49153, 32769), 20000, 0, 17000),
 ]
 
 

@@ -145,8 +145,9 @@ def test_evict_checks(over, code):
 
 def test_evict_workspace():
     L = _lib.lib()
-    need = L.fa_paged_evict_workspace_bytes(2, 8, 64)
-    assert need == 2 * 8 * 64 * 4 and L.fa_paged_evict_workspace_bytes(0, 8, 64) == 0
+    need = L.fa_paged_evict_workspace_bytes(2, 8, 64, 160)
+    assert need == 2 * 8 * 64 * 4 and L.fa_paged_evict_workspace_bytes(0, 8, 64, 160) == 0
+    assert L.fa_paged_evict_workspace_bytes(2, 8, 64, 1 << 17) > need  # (several workgroups a head)
     for ws, n in ((None, need), (FAKE + 16, need), (FAKE, need - 1)):
         assert L.fa_paged_evict(ctypes.byref(_evict()), ws, n, None) == _code("WORKSPACE")
 
