@@ -65,10 +65,11 @@ fa::PagedCache cache_args(const fa_paged_cache& c) {
 
 int status(hipError_t e) { return e == hipSuccess ? FA_OK : FA_ERR_LAUNCH; }
 
-// Sequences of at most this many visible keys are taken whole, a workgroup each, in one launch.
-constexpr int kWholeKeys = 512;
+// Sequences of at most so many visible keys are taken whole, a workgroup each, in one launch: kWholeKeys, or kWholeMany
+// where there are at least kManyWgs (KV head, row tile, sequence) triples.
+constexpr int kWholeKeys = 1024, kWholeMany = 2048, kManyWgs = 128;
 // Workgroups of a split call's launch for each compute unit, and the fewest units worth a workgroup of their own.
-constexpr int kPartsPerCu = 2, kLeastUnits = 2;
+constexpr int kPartsPerCu = 2, kLeastUnits = 1;
 
 // K and V bytes up to which a call's loads leave them in the 256 MB last-level cache, for the next step to find.
 constexpr int64_t kKeepBytes = int64_t(96) << 20;
@@ -107,7 +108,7 @@ int plan(const fa_paged_attention_params* p, Plan* r) {
   const int64_t streams = int64_t(c.heads_kv) * r->row_tiles, units = int64_t(c.batch) * r->max_units;
   if (units >= (int64_t(1) << 31) || !fa::grid_fits(std::max(streams, int64_t(p->heads_q)) * c.batch)) return FA_ERR_OVERFLOW;
   r->parts = 0;
-  if (most > kWholeKeys) {
+  if (most > (streams * c.batch >= kManyWgs ? kWholeMany : kWholeKeys)) {
     const int64_t want = std::max<int64_t>(1, int64_t(kPartsPerCu) * fa::device_cus() / streams);
     // (whole rounds of the 8 XCDs: the tiles of a group's heads then read the same keys through one L2)
     r->parts = int((std::min(want, (units + kLeastUnits - 1) / kLeastUnits) + 7) / 8 * 8);
@@ -217,6 +218,7 @@ int fa_paged_attention(const fa_paged_attention_params* p, void* workspace, size
   a.max_units = r.max_units;
   a.parts = r.parts;
   a.least = kLeastUnits;
+  a.wide = !r.parts && int64_t(c.heads_kv) * r.row_tiles * c.batch <= fa::device_cus();
   a.keep_units = int(std::min<int64_t>(kKeepBytes / (int64_t(fa::kPagedUnit) * 2 * c.head_dim * elem_bytes(c.dtype) * c.heads_kv), INT32_MAX));
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   a.part_o = reinterpret_cast<float*>(ws);

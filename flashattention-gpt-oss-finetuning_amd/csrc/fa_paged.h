@@ -46,6 +46,7 @@ struct PagedAttnArgs {
   int max_units;          // units of a sequence of max_len tokens
   // split calls: the runs a (KV head, row tile) is cut into, 0 where every workgroup takes a whole sequence
   int parts, least;
+  int wide;               // 8 waves a workgroup instead of 4
   int keep_units;         // calls that read more units a KV head than this mark their loads as read once
   // workspace
   float* part_o;          // [Hkv row_tiles][parts][2][16][D]

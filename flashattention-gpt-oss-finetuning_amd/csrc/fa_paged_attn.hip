@@ -4,7 +4,7 @@
 //     s[h, k] = scale q[h] . K[k],   lse[h] = log(sum_k exp s[h, k] + exp(sink[h])),   o[h] = sum_k exp(s[h, k] - lse[h]) V[k].
 // 4 G operations a cache element, so the cache's bytes bound it: the kernel is built to keep them coming.
 //
-// paged_attn_kernel.  A workgroup of 4 waves takes a run of keys for 16 query heads (a group, padded); its waves
+// paged_attn_kernel.  A workgroup of 4 or 8 waves takes a run of keys for 16 query heads (a group, padded); its waves
 // take tiles of 32 keys in turn and meet only at the run's end.  A tile goes from memory to registers to the
 // matrix instructions, without LDS and without a lane seeing another's values:
 //   * S^T = K Q^T as v_mfma_f32_16x16x32 with the keys as rows.  Lane l (r = l % 16, j = l / 16) supplies key rows r of two
@@ -38,7 +38,6 @@ namespace fa {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kWaves = 4;
 constexpr int kTile = 32;
 
 __device__ __forceinline__ int seq_len(const PagedCache& c, int b) { return imin(imax(c.lens[b], 0), c.max_len); }
@@ -138,6 +137,7 @@ struct Tile {
   static constexpr int NK = STAGED ? PR / 2 : 2 * NF;        // pieces of the tile that a lane loads
   static constexpr int VB = ROW / 16;                        // bytes of a V entry that a lane holds
   static constexpr int VD = VB >= 4 ? VB / 4 : 1;
+  static constexpr int AHEAD = ROW <= 64 ? 4 : 2;  // tiles in flight, of 4 to 64 registers each way
   u32x4 k[NK];
   uint32_t v[8][VD];
   uint32_t live;  // bit i: key i of the tile is on a page (the same in every lane)
@@ -386,7 +386,7 @@ struct No {
   static constexpr bool value = false;
 };
 
-template <typename E, int D>
+template <typename E, int D, int WAVES>
 struct Shared {
   static constexpr int PAD = D + 4;  // float32 rows 4 banks apart
   union {
@@ -395,16 +395,16 @@ struct Shared {
         int64_t k[64], v[64];
       } off[2];
       u32x4 k[Tile<E, D>::STAGED ? kTile * Tile<E, D>::PR : 1];
-    } wave[kWaves];
-    float o[kWaves][16][PAD];
+    } wave[WAVES];
+    float o[WAVES][16][PAD];
   };
-  float m[kWaves][16], l[kWaves][16];
+  float m[WAVES][16], l[WAVES][16];
 };
 
-template <typename E, int D>
-__global__ __launch_bounds__(kThreads) void paged_attn_kernel(const PagedAttnArgs a) {
+template <typename E, int D, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void paged_attn_kernel(const PagedAttnArgs a) {
   constexpr int NC = D / 16;
-  __shared__ Shared<E, D> sh;
+  __shared__ Shared<E, D, WAVES> sh;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 15, j = lane >> 4;
   const int parts = a.parts ? a.parts : a.c.B;
@@ -446,11 +446,11 @@ __global__ __launch_bounds__(kThreads) void paged_attn_kernel(const PagedAttnArg
     w.load_q(a.q + int64_t(b) * a.sq[0] + int64_t(r < heads ? head : hkv * a.G) * a.sq[1], r < heads);
     w.reset();
     const int* table = a.c.table + int64_t(b) * a.c.table_stride;
-    // The wave's tiles, in pairs: tiles wave + 8p and wave + 8p + 4 of the run.  A lane works out the place of one of a
-    // pair's 64 keys: its page is asked for two pairs ahead, its offsets are in LDS one pair ahead.
-    const int n = v1 - v0, tiles = (n + kTile - 1) / kTile, mine = (tiles - wave + kWaves - 1) / kWaves, pairs = (mine + 1) / 2;
+    // The wave's tiles are every 4th (8th) of the run.  A lane works out the place of one of the 64 keys of two of them (a
+    // pair): its page is asked for one pair ahead of its offsets, which go to LDS just before the loads that use them.
+    const int n = v1 - v0, tiles = (n + kTile - 1) / kTile, mine = (tiles - wave + WAVES - 1) / WAVES;
     auto ask = [&](int p, int& slot) {
-      const int v = (wave + kWaves * (2 * p + (lane >> 5))) * kTile + (lane & 31);
+      const int v = (wave + WAVES * (2 * p + (lane >> 5))) * kTile + (lane & 31);
       slot = 0;
       if (v >= n) return -1;
       const int key = visible_key(vis, v0 + v), pi = page_of(a.c.div, key);
@@ -468,29 +468,37 @@ __global__ __launch_bounds__(kThreads) void paged_attn_kernel(const PagedAttnArg
     };
     auto logits = [&](int i) -> float* {  // of the wave's i-th tile
       if (!a.sums || r >= heads) return nullptr;
-      const int at = v0 + (wave + kWaves * i) * kTile;
+      const int at = v0 + (wave + WAVES * i) * kTile;
       return a.logits + (((int64_t(hkv) * a.c.B + b) * a.max_units + at / kPagedUnit) * a.G + h0 + r) * kPagedUnit + at % kPagedUnit +
              8 * j;
     };
     auto walk = [&](auto mode) {
       constexpr bool ONCE = decltype(mode)::value;
-      auto& off = sh.wave[wave].off;
+      constexpr int AHEAD = Tile<E, D>::AHEAD;
+      Tile<E, D> t[AHEAD];
+      unsigned long long live = 0;
       int slot, page = ask(0, slot);
-      unsigned long long live = place(0, page, slot);
-      page = ask(1, slot);
-      Tile<E, D> t, next;
-      w.template load<ONCE>(t, kb, vb, off[0].k, off[0].v, uint32_t(live));
-      for (int p = 0; p < pairs; ++p) {
-        const bool two = 2 * p + 1 < mine;
-        if (two) w.template load<ONCE>(next, kb, vb, off[p & 1].k + kTile, off[p & 1].v + kTile, uint32_t(live >> 32));
-        live = place(p + 1, page, slot);
-        page = ask(p + 2, slot);
-        w.step(t, a.c2, sh.wave[wave].k, logits(2 * p));
-        if (p + 1 < pairs) w.template load<ONCE>(t, kb, vb, off[(p + 1) & 1].k, off[(p + 1) & 1].v, uint32_t(live));
-        if (two) w.step(next, a.c2, sh.wave[wave].k, logits(2 * p + 1));
+      auto load = [&](Tile<E, D>& to, int i, bool first) {  // the wave's i-th tile; `first` of its pair
+        if (i >= mine) return;
+        const int p = i >> 1;
+        if (first) {
+          live = place(p, page, slot);
+          page = ask(p + 1, slot);
+        }
+        const auto& off = sh.wave[wave].off[p & 1];
+        w.template load<ONCE>(to, kb, vb, off.k + (first ? 0 : kTile), off.v + (first ? 0 : kTile), uint32_t(first ? live : live >> 32));
+      };
+#pragma unroll
+      for (int d = 0; d < AHEAD; ++d) load(t[d], d, d % 2 == 0);
+      for (int i = 0; i < mine; i += AHEAD) {
+#pragma unroll
+        for (int d = 0; d < AHEAD; ++d) {
+          if (i + d < mine) w.step(t[d], a.c2, sh.wave[wave].k, logits(i + d));
+          load(t[d], i + d + AHEAD, d % 2 == 0);
+        }
       }
     };
-    if (pairs > 0) {
+    if (mine > 0) {
       if (once) walk(Yes{});
       else walk(No{});
     }
@@ -510,17 +518,17 @@ __global__ __launch_bounds__(kThreads) void paged_attn_kernel(const PagedAttnArg
     const int oh = tid >> 4, od = (tid & 15) * NC;  // this thread's head and dims
     float m = kNegInf;
 #pragma unroll
-    for (int x = 0; x < kWaves; ++x) m = fmaxf(m, sh.m[x][oh]);
+    for (int x = 0; x < WAVES; ++x) m = fmaxf(m, sh.m[x][oh]);
     const float ref = m == kNegInf ? 0.f : m;
     float sum = 0.f, o[NC] = {};
 #pragma unroll
-    for (int x = 0; x < kWaves; ++x) {
+    for (int x = 0; x < WAVES; ++x) {
       const float f = fast_exp2(sh.m[x][oh] - ref);
       sum += f * sh.l[x][oh];
 #pragma unroll
       for (int c = 0; c < NC; ++c) o[c] += f * sh.o[x][oh][od + c];
     }
-    if (oh < heads) {
+    if (oh < heads) {  // (with 8 waves, the first 4)
       const int hq = hkv * a.G + h0 + oh;
       if (whole) {
         float ls = sum, scale = 1.f;
@@ -617,18 +625,26 @@ __device__ __forceinline__ void join_head(const PagedAttnArgs& a, int b, int hq,
 // sums[b, hkv, key] += sum over the group's heads of 2^(logit - lse): a thread takes keys, so there is no order to choose and
 // no atomic.
 constexpr int kSumKeys = 1024;
-constexpr int kSumHeads = 64;  // heads whose lse a workgroup holds at a time
+constexpr int kSumHeads = 16;  // heads at a time: 16 threads work out a head's lse
 __device__ __forceinline__ void add_weights(const PagedAttnArgs& a, int b, int hkv, int chunk, float* smem) {
   const Visible vis = visible(seq_len(a.c, b), a.W, a.S);
-  const int v0 = chunk * kSumKeys + 4 * int(threadIdx.x);
   if (chunk * kSumKeys >= vis.count) return;
+  // (a thread past the last key reads the last unit's room and writes nothing)
+  const int v0 = chunk * kSumKeys + 4 * int(threadIdx.x), vr = imin(v0, (vis.count - 1) / 4 * 4);
+  const float* x = a.logits + ((int64_t(hkv) * a.c.B + b) * a.max_units + vr / kPagedUnit) * a.G * kPagedUnit + vr % kPagedUnit;
+  float* out = a.sums + int64_t(b) * a.ssum[0] + int64_t(hkv) * a.ssum[1];
+  float w[4] = {0.f, 0.f, 0.f, 0.f}, old[4];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) old[c] = out[visible_key(vis, imin(v0 + c, vis.count - 1))];
   const Pieces ps = pieces_of(a, b);
-  float w[4] = {0.f, 0.f, 0.f, 0.f};
   for (int g0 = 0; g0 < a.G; g0 += kSumHeads) {
     const int ng = imin(kSumHeads, a.G - g0);
+    constexpr int HELD = 8;  // scores asked for before the lse are known
+    f32x4 s[HELD];
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) s[i] = *reinterpret_cast<const f32x4*>(x + (g0 + imin(i, ng - 1)) * kPagedUnit);
     if (g0) __syncthreads();
-    // four threads work out a head's lse
-    const int g = g0 + int(threadIdx.x) / 4, sub = threadIdx.x & 3;
+    const int g = g0 + int(threadIdx.x) / 16, sub = threadIdx.x & 15;
     if (g < a.G) {
       const int hq = hkv * a.G + g;
       float lse;
@@ -638,38 +654,35 @@ __device__ __forceinline__ void add_weights(const PagedAttnArgs& a, int b, int h
         const float* ml = a.part_ml + int64_t(hkv * a.row_tiles + g / 16) * a.parts * 2 * 32 + g % 16;
         float m = a.sinks ? a.sinks[hq] * kLog2e : kNegInf;
         const float sink = m;
-        for (int p = ps.first + sub; p <= ps.last; p += 4) m = fmaxf(m, ml[part_slot(p, ps.per, ps.start) * 32]);
-        m = fmaxf(m, __shfl_xor(m, 1));
-        m = fmaxf(m, __shfl_xor(m, 2));
+        for (int p = ps.first + sub; p <= ps.last; p += 16) m = fmaxf(m, ml[part_slot(p, ps.per, ps.start) * 32]);
+#pragma unroll
+        for (int y = 8; y >= 1; y >>= 1) m = fmaxf(m, __shfl_xor(m, y));
         const float ref = m == kNegInf ? 0.f : m;
-        float s = sub == 0 && sink != kNegInf ? fast_exp2(sink - ref) : 0.f;
-        for (int p = ps.first + sub; p <= ps.last; p += 4) {
+        float l = sub == 0 && sink != kNegInf ? fast_exp2(sink - ref) : 0.f;
+        for (int p = ps.first + sub; p <= ps.last; p += 16) {
           const int slot = part_slot(p, ps.per, ps.start) * 32;
-          s += fast_exp2(ml[slot] - ref) * ml[slot + 16];
+          l += fast_exp2(ml[slot] - ref) * ml[slot + 16];
         }
-        s += __shfl_xor(s, 1);
-        s += __shfl_xor(s, 2);
-        lse = ref + fast_log2(s);
+#pragma unroll
+        for (int y = 8; y >= 1; y >>= 1) l += __shfl_xor(l, y);
+        lse = ref + fast_log2(l);
       }
       if (sub == 0) smem[g - g0] = lse;
     }
     __syncthreads();
-    if (v0 < vis.count) {
-      const float* x = a.logits +
-                       ((int64_t(hkv) * a.c.B + b) * a.max_units + v0 / kPagedUnit) * a.G * kPagedUnit + g0 * kPagedUnit + v0 % kPagedUnit;
-#pragma unroll 8
-      for (int i = 0; i < ng; ++i) {
-        const f32x4 s = *reinterpret_cast<const f32x4*>(x + i * kPagedUnit);
-        const float lse = smem[i];
+    auto add = [&](f32x4 q, int i) {
+      const float lse = smem[i];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) w[c] += s[c] == kNegInf ? 0.f : fast_exp2(s[c] - lse);
-      }
-    }
+      for (int c = 0; c < 4; ++c) w[c] += q[c] == kNegInf ? 0.f : fast_exp2(q[c] - lse);
+    };
+#pragma unroll
+    for (int i = 0; i < HELD; ++i)
+      if (i < ng) add(s[i], i);
+    for (int i = HELD; i < ng; ++i) add(*reinterpret_cast<const f32x4*>(x + (g0 + i) * kPagedUnit), i);
   }
-  float* out = a.sums + int64_t(b) * a.ssum[0] + int64_t(hkv) * a.ssum[1];
 #pragma unroll
   for (int c = 0; c < 4; ++c)
-    if (v0 + c < vis.count) out[visible_key(vis, v0 + c)] += w[c];
+    if (v0 + c < vis.count) out[visible_key(vis, v0 + c)] = old[c] + w[c];
 }
 
 // Workgroups [0, joins) join heads, the ones behind them add weights.
@@ -687,7 +700,14 @@ __global__ __launch_bounds__(kThreads) void paged_finish_kernel(const PagedAttnA
 template <typename E, int D>
 hipError_t run(const PagedAttnArgs& a, hipStream_t s) {
   const unsigned streams = unsigned(a.c.Hkv * a.row_tiles), B = unsigned(a.c.B);
-  hipLaunchKernelGGL((paged_attn_kernel<E, D>), dim3(streams * (a.parts ? unsigned(a.parts) : B)), dim3(kThreads), 0, s, a);
+  const dim3 grid(streams * (a.parts ? unsigned(a.parts) : B));
+  // 8 waves where the workgroups are few and the waves' tables and tiles fit the 64 KB of LDS
+  if constexpr (sizeof(Shared<E, D, 8>) <= 65536) {
+    if (!a.wide) hipLaunchKernelGGL((paged_attn_kernel<E, D, 4>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((paged_attn_kernel<E, D, 8>), grid, dim3(512), 0, s, a);
+  } else {
+    hipLaunchKernelGGL((paged_attn_kernel<E, D, 4>), grid, dim3(256), 0, s, a);
+  }
   const hipError_t e = hipGetLastError();
   const unsigned joins = a.parts ? unsigned(a.Hq) * B : 0u;
   const unsigned adds = a.sums ? unsigned((a.max_units * kPagedUnit + kSumKeys - 1) / kSumKeys) * unsigned(a.c.Hkv) * B : 0u;
