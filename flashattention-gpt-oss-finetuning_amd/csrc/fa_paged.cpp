@@ -68,14 +68,18 @@ int status(hipError_t e) { return e == hipSuccess ? FA_OK : FA_ERR_LAUNCH; }
 // Sequences of at most so many visible keys are taken whole, a workgroup each, in one launch: kWholeKeys, or kWholeMany
 // where there are at least kManyWgs (KV head, row tile, sequence) triples.
 constexpr int kWholeKeys = 1024, kWholeMany = 2048, kManyWgs = 128;
-// Workgroups of a split call's launch for each compute unit, and the fewest units worth a workgroup of their own.
-constexpr int kPartsPerCu = 2, kLeastUnits = 1;
+// Workgroups of a split call's launch for each compute unit (more for rows of 32 bytes, whose tiles are as much work and a
+// quarter of the bytes of D = 64), and the fewest units worth a workgroup of their own.
+constexpr int kPartsPerCu = 2, kPartsNarrow = 3, kLeastUnits = 1;
+
+// Whole sequences of at most kSingleUnits units are taken by one wave each where there are kSingleWgs of them.
+constexpr int kSingleWgs = 1024, kSingleUnits = 2;
 
 // K and V bytes up to which a call's loads leave them in the 256 MB last-level cache, for the next step to find.
 constexpr int64_t kKeepBytes = int64_t(96) << 20;
 
 struct Plan {
-  int max_units, row_tiles, parts;
+  int max_units, row_tiles, rt, parts;
   size_t part_o, part_ml, lse, logits;  // bytes
   size_t bytes() const { return std::max<size_t>(256, part_o + part_ml + lse + logits); }
 };
@@ -105,16 +109,17 @@ int plan(const fa_paged_attention_params* p, Plan* r) {
   const int G = p->heads_q / c.heads_kv;
   r->max_units = fa::paged_units(int(most));
   r->row_tiles = (G + 15) / 16;
-  const int64_t streams = int64_t(c.heads_kv) * r->row_tiles, units = int64_t(c.batch) * r->max_units;
+  r->rt = r->row_tiles > 1 && fa::paged_pairs(c.head_dim, elem_bytes(c.dtype)) ? 2 : 1;
+  const int64_t streams = int64_t(c.heads_kv) * ((r->row_tiles + r->rt - 1) / r->rt), units = int64_t(c.batch) * r->max_units;
   if (units >= (int64_t(1) << 31) || !fa::grid_fits(std::max(streams, int64_t(p->heads_q)) * c.batch)) return FA_ERR_OVERFLOW;
   r->parts = 0;
   if (most > (streams * c.batch >= kManyWgs ? kWholeMany : kWholeKeys)) {
-    const int64_t want = std::max<int64_t>(1, int64_t(kPartsPerCu) * fa::device_cus() / streams);
+    const int64_t want = std::max<int64_t>(1, int64_t(c.head_dim * elem_bytes(c.dtype) <= 32 ? kPartsNarrow : kPartsPerCu) * fa::device_cus() / streams);
     // (whole rounds of the 8 XCDs: the tiles of a group's heads then read the same keys through one L2)
     r->parts = int((std::min(want, (units + kLeastUnits - 1) / kLeastUnits) + 7) / 8 * 8);
     if (!fa::grid_fits(streams * r->parts)) return FA_ERR_OVERFLOW;
   }
-  const size_t slots = size_t(streams) * r->parts * 2;
+  const size_t slots = size_t(c.heads_kv) * r->row_tiles * r->parts * 2;
   r->part_o = align256(slots * 16 * c.head_dim * sizeof(float));
   r->part_ml = align256(slots * 32 * sizeof(float));
   r->lse = r->logits = 0;
@@ -211,6 +216,7 @@ int fa_paged_attention(const fa_paged_attention_params* p, void* workspace, size
   a.Hq = p->heads_q;
   a.G = p->heads_q / c.heads_kv;
   a.row_tiles = r.row_tiles;
+  a.rt = r.rt;
   a.W = std::min(std::max(p->window, 0), a.c.max_len);
   a.S = std::min(std::max(p->sink, 0), a.c.max_len);
   a.c2 = float(double(p->softmax_scale) * 1.4426950408889634 * (q8 ? c.k_descale : 1.0));
@@ -218,7 +224,8 @@ int fa_paged_attention(const fa_paged_attention_params* p, void* workspace, size
   a.max_units = r.max_units;
   a.parts = r.parts;
   a.least = kLeastUnits;
-  a.wide = !r.parts && int64_t(c.heads_kv) * r.row_tiles * c.batch <= fa::device_cus();
+  const int64_t wgs = int64_t(c.heads_kv) * r.row_tiles * c.batch;
+  a.waves = r.parts ? 4 : wgs <= fa::device_cus() ? 8 : wgs >= kSingleWgs && r.max_units <= kSingleUnits ? 1 : 4;
   a.keep_units = int(std::min<int64_t>(kKeepBytes / (int64_t(fa::kPagedUnit) * 2 * c.head_dim * elem_bytes(c.dtype) * c.heads_kv), INT32_MAX));
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   a.part_o = reinterpret_cast<float*>(ws);

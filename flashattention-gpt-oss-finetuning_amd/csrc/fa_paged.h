@@ -31,6 +31,9 @@ struct AppendArgs {
   float k_inv, v_inv;     // e4m3 pages: reciprocals of the descales
 };
 
+// Two tiles of heads and their sums fit a wave's registers: more than 16 heads a group then share what is read.
+constexpr bool paged_pairs(int D, int cache_bytes) { return cache_bytes <= 2 && D * cache_bytes <= 128; }
+
 struct PagedAttnArgs {
   PagedCache c;
   const uint8_t* q;
@@ -46,7 +49,8 @@ struct PagedAttnArgs {
   int max_units;          // units of a sequence of max_len tokens
   // split calls: the runs a (KV head, row tile) is cut into, 0 where every workgroup takes a whole sequence
   int parts, least;
-  int wide;               // 8 waves a workgroup instead of 4
+  int waves;              // of a workgroup: 1, 4 or 8
+  int rt;                 // tiles of heads that a workgroup takes: 1, or 2 (paged_pairs)
   int keep_units;         // calls that read more units a KV head than this mark their loads as read once
   // workspace
   float* part_o;          // [Hkv row_tiles][parts][2][16][D]

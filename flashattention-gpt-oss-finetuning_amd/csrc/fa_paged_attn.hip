@@ -143,32 +143,36 @@ struct Tile {
   uint32_t live;  // bit i: key i of the tile is on a page (the same in every lane)
 };
 
-template <typename E, int D>
+// A wave's state for RT tiles of 16 heads, which share the key tiles that it reads.
+template <typename E, int D, int RT>
 struct Wave {
   using T = Tile<E, D>;
   static constexpr int NC = D / 16;                          // dims a lane of the output holds of each 16 rows
   static constexpr bool F = E::EB == 4;
   static constexpr int NQ = F ? D / 16 : (D >= 32 ? D / 32 : 1);
-  u32x4 q[NQ];
-  f32x4 acc[NC];
-  float m, mref, l;  // running maximum (log2 domain), the same with 0 for none, this lane's sum
+  u32x4 q[RT][NQ];
+  f32x4 acc[RT][NC];
+  float m[RT], mref[RT], l[RT];  // running maximum (log2 domain), the same with 0 for none, this lane's sum
 
   // Q as the B operand: head r of the tile, dims in the order in which the K pieces hold them.
-  __device__ __forceinline__ void load_q(const uint8_t* q_row, bool have) {
+  __device__ __forceinline__ void load_q(int x, const uint8_t* q_row, bool have) {
     const int j = (threadIdx.x & 63) >> 4;
 #pragma unroll
     for (int f = 0; f < NQ; ++f) {
       // 16-byte piece 4f + j of the row; an e4m3 piece holds 16 dims, two pieces of q
       const int piece = E::CB == 1 ? 2 * (4 * (f / 2) + j) + f % 2 : 4 * f + j;
-      q[f] = have && piece * 16 < D * E::EB ? ld16(q_row + 16 * piece) : zero16();
+      q[x][f] = have && piece * 16 < D * E::EB ? ld16(q_row + 16 * piece) : zero16();
     }
   }
   __device__ __forceinline__ void reset() {
 #pragma unroll
-    for (int c = 0; c < NC; ++c) acc[c] = f32x4{0.f, 0.f, 0.f, 0.f};
-    m = kNegInf;
-    mref = 0.f;
-    l = 0.f;
+    for (int x = 0; x < RT; ++x) {
+#pragma unroll
+      for (int c = 0; c < NC; ++c) acc[x][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+      m[x] = kNegInf;
+      mref[x] = 0.f;
+      l[x] = 0.f;
+    }
   }
 
   // koff, voff: the tile's 32 offsets of K, and of V, in LDS.
@@ -228,10 +232,10 @@ struct Wave {
     return row * PR + (p ^ s);
   }
 
-  // lds: the wave's room for a staged K tile; logits: where the lane's eight scores go, or NULL
-  __device__ __forceinline__ void step(T& t, float c2, u32x4* lds, float* logits) {
+  // lds: the wave's room for a staged K tile; logits(x): where the lane's eight scores of head tile x go, or NULL
+  template <typename L>
+  __device__ __forceinline__ void step(T& t, float c2, u32x4* lds, L&& logits) {
     const int lane = threadIdx.x & 63, r = lane & 15, j = lane >> 4;
-    f32x4 s0 = {0.f, 0.f, 0.f, 0.f}, s1 = s0;
     u32x4 kf[2][T::NF];
     if constexpr (T::STAGED) {
 #pragma unroll
@@ -247,19 +251,29 @@ struct Wave {
 #pragma unroll
       for (int n = 0; n < 2 * T::NF; ++n) kf[n / T::NF][n % T::NF] = t.k[n];
     }
-    if constexpr (F) {
+    if (t.live != ~0u) {
 #pragma unroll
-      for (int n = 0; n < T::NF; ++n)
+      for (int e = 0; e < 8; ++e) {
+        const bool ok = t.live >> (8 * j + e) & 1;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint32_t k0 = kf[0][n][e], k1 = kf[1][n][e], qe = q[n][e];
-          s0 = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, k0), __builtin_bit_cast(float, qe), s0, 0, 0, 0);
-          s1 = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, k1), __builtin_bit_cast(float, qe), s1, 0, 0, 0);
-        }
-    } else {
+        for (int w = 0; w < T::VD; ++w) t.v[e][w] = ok ? t.v[e][w] : 0u;
+      }
+    }
+    u32x4 hi[RT], lo[RT];  // the weights as B operands, in two 16-bit parts
+    float p[RT][8];
+#pragma unroll
+    for (int x = 0; x < RT; ++x) {
+      f32x4 s0 = {0.f, 0.f, 0.f, 0.f}, s1 = s0;
 #pragma unroll
       for (int n = 0; n < T::NF; ++n) {
-        if constexpr (E::CB == 1) {
+        if constexpr (F) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t k0 = kf[0][n][e], k1 = kf[1][n][e], qe = q[x][n][e];
+            s0 = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, k0), __builtin_bit_cast(float, qe), s0, 0, 0, 0);
+            s1 = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, k1), __builtin_bit_cast(float, qe), s1, 0, 0, 0);
+          }
+        } else if constexpr (E::CB == 1) {
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
             u32x4 k0, k1;
@@ -270,87 +284,82 @@ struct Wave {
               k1[2 * w] = E::widen(kf[1][n][2 * u + w], false);
               k1[2 * w + 1] = E::widen(kf[1][n][2 * u + w], true);
             }
-            s0 = E::mfma16(k0, q[2 * n + u], s0);
-            s1 = E::mfma16(k1, q[2 * n + u], s1);
+            s0 = E::mfma16(k0, q[x][2 * n + u], s0);
+            s1 = E::mfma16(k1, q[x][2 * n + u], s1);
           }
         } else {
-          s0 = E::mfma16(kf[0][n], q[n], s0);
-          s1 = E::mfma16(kf[1][n], q[n], s1);
+          s0 = E::mfma16(kf[0][n], q[x][n], s0);
+          s1 = E::mfma16(kf[1][n], q[x][n], s1);
         }
       }
-    }
-    float s[8];
+      float s[8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      s[i] = s0[i] * c2;
-      s[4 + i] = s1[i] * c2;
-    }
-    if (t.live != ~0u) {
+      for (int i = 0; i < 4; ++i) {
+        s[i] = s0[i] * c2;
+        s[4 + i] = s1[i] * c2;
+      }
+      if (t.live != ~0u) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[e] = t.live >> (8 * j + e) & 1 ? s[e] : kNegInf;
+      }
+      if (float* to = logits(x)) {
+        *reinterpret_cast<f32x4*>(to) = f32x4{s[0], s[1], s[2], s[3]};
+        *reinterpret_cast<f32x4*>(to + 4) = f32x4{s[4], s[5], s[6], s[7]};
+      }
+      float mx = s[0];
+#pragma unroll
+      for (int e = 1; e < 8; ++e) mx = fmaxf(mx, s[e]);
+      if (wave_any(mx > m[x] + 8.f)) {
+        const float up = fmaxf(m[x], quarters_max(mx));
+        const float scale = m[x] == kNegInf ? 0.f : fast_exp2(m[x] - up);
+        l[x] *= scale;
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[x][c][i] *= scale;
+        m[x] = up;
+        mref[x] = up == kNegInf ? 0.f : up;
+      }
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const bool ok = t.live >> (8 * j + e) & 1;
-        s[e] = ok ? s[e] : kNegInf;
-#pragma unroll
-        for (int w = 0; w < T::VD; ++w) t.v[e][w] = ok ? t.v[e][w] : 0u;
+        p[x][e] = fast_exp2(s[e] - mref[x]);
+        l[x] += p[x][e];
       }
-    }
-    if (logits) {
-      *reinterpret_cast<f32x4*>(logits) = f32x4{s[0], s[1], s[2], s[3]};
-      *reinterpret_cast<f32x4*>(logits + 4) = f32x4{s[4], s[5], s[6], s[7]};
-    }
-    float mx = s[0];
+      if constexpr (!F) {
+        hi[x] = pack8<E>(p[x]);
+        float rest[8];
 #pragma unroll
-    for (int e = 1; e < 8; ++e) mx = fmaxf(mx, s[e]);
-    if (wave_any(mx > m + 8.f)) {
-      const float up = fmaxf(m, quarters_max(mx));
-      const float scale = m == kNegInf ? 0.f : fast_exp2(m - up);
-      l *= scale;
-#pragma unroll
-      for (int c = 0; c < NC; ++c)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[c][i] *= scale;
-      m = up;
-      mref = m == kNegInf ? 0.f : m;
-    }
-    float p[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      p[e] = fast_exp2(s[e] - mref);
-      l += p[e];
+        for (int w = 0; w < 4; ++w) {
+          rest[2 * w] = p[x][2 * w] - E::to_f32(uint16_t(hi[x][w]));
+          rest[2 * w + 1] = p[x][2 * w + 1] - E::to_f32(uint16_t(hi[x][w] >> 16));
+        }
+        lo[x] = pack8<E>(rest);
+      }
     }
     if constexpr (F) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-#pragma unroll
-        for (int c = 0; c < NC; ++c)
-          acc[c] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, t.v[e][c]), p[e], acc[c], 0, 0, 0);
-    } else {
-      const u32x4 hi = pack8<E>(p);
-      float rest[8];
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        rest[2 * w] = p[2 * w] - E::to_f32(uint16_t(hi[w]));
-        rest[2 * w + 1] = p[2 * w + 1] - E::to_f32(uint16_t(hi[w] >> 16));
-      }
-      const u32x4 lo = pack8<E>(rest);
-      if constexpr (E::CB == 1) {
-        uint32_t w[8][NC / 2];
+      for (int x = 0; x < RT; ++x)
 #pragma unroll
         for (int e = 0; e < 8; ++e)
 #pragma unroll
-          for (int d = 0; d < NC / 2; ++d) w[e][d] = E::widen(t.v[e][d / 2], d % 2);
+          for (int c = 0; c < NC; ++c)
+            acc[x][c] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, t.v[e][c]), p[x][e], acc[x][c], 0, 0, 0);
+    } else {
+      uint32_t w[8][NC >= 2 ? NC / 2 : 1];
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-          const u32x4 f = v_frag(w, c);
-          acc[c] = E::mfma16(f, hi, acc[c]);
-          acc[c] = E::mfma16(f, lo, acc[c]);
+      for (int e = 0; e < 8; ++e)
+#pragma unroll
+        for (int d = 0; d < (NC >= 2 ? NC / 2 : 1); ++d) {
+          if constexpr (E::CB == 1) w[e][d] = E::widen(t.v[e][d / 2], d % 2);
+          else w[e][d] = t.v[e][d];
         }
-      } else {
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-          const u32x4 f = v_frag(t.v, c);
-          acc[c] = E::mfma16(f, hi, acc[c]);
-          acc[c] = E::mfma16(f, lo, acc[c]);
+      for (int c = 0; c < NC; ++c) {
+        const u32x4 f = v_frag(w, c);
+#pragma unroll
+        for (int x = 0; x < RT; ++x) {
+          acc[x][c] = E::mfma16(f, hi[x], acc[x][c]);
+          acc[x][c] = E::mfma16(f, lo[x], acc[x][c]);
         }
       }
     }
@@ -401,7 +410,7 @@ struct Shared {
   float m[WAVES][16], l[WAVES][16];
 };
 
-template <typename E, int D, int WAVES>
+template <typename E, int D, int WAVES, int RT>
 __global__ __launch_bounds__(64 * WAVES) void paged_attn_kernel(const PagedAttnArgs a) {
   constexpr int NC = D / 16;
   __shared__ Shared<E, D, WAVES> sh;
@@ -409,8 +418,8 @@ __global__ __launch_bounds__(64 * WAVES) void paged_attn_kernel(const PagedAttnA
   const int r = lane & 15, j = lane >> 4;
   const int parts = a.parts ? a.parts : a.c.B;
   const int stream = blockIdx.x / parts, part = blockIdx.x % parts;
-  const int hkv = stream / a.row_tiles, h0 = stream % a.row_tiles * 16;  // first head of the tile within the group
-  const int heads = imin(16, a.G - h0);
+  const int shares = (a.row_tiles + RT - 1) / RT;  // workgroups that a group's heads are shared out to
+  const int hkv = stream / shares, h0 = stream % shares * (16 * RT);  // first head within the group
   const uint8_t* kb = a.c.k + int64_t(hkv) * a.c.sk[1];
   const uint8_t* vb = a.c.v + int64_t(hkv) * a.c.sv[1];
 
@@ -432,7 +441,7 @@ __global__ __launch_bounds__(64 * WAVES) void paged_attn_kernel(const PagedAttnA
     find_unit(a, u, b, start);
   }
 
-  Wave<E, D> w;
+  Wave<E, D, RT> w;
   // (b < B, v0 >= 0 and the join's last part hold by themselves, unless lens change under a running call: then the results
   // mean nothing, but no access leaves the tensors)
   while (u < end && b < a.c.B) {
@@ -442,8 +451,11 @@ __global__ __launch_bounds__(64 * WAVES) void paged_attn_kernel(const PagedAttnA
     const int stop = imin(end, start + units);
     const bool whole = u == start && stop == start + units;
     const int v0 = imax(0, (u - start) * kPagedUnit), v1 = imin(vis.count, (stop - start) * kPagedUnit);
-    const int head = hkv * a.G + h0 + r;
-    w.load_q(a.q + int64_t(b) * a.sq[0] + int64_t(r < heads ? head : hkv * a.G) * a.sq[1], r < heads);
+#pragma unroll
+    for (int x = 0; x < RT; ++x) {
+      const int h = h0 + 16 * x + r;
+      w.load_q(x, a.q + int64_t(b) * a.sq[0] + int64_t(hkv * a.G + (h < a.G ? h : 0)) * a.sq[1], h < a.G);
+    }
     w.reset();
     const int* table = a.c.table + int64_t(b) * a.c.table_stride;
     // The wave's tiles are every 4th (8th) of the run.  A lane works out the place of one of the 64 keys of two of them (a
@@ -466,11 +478,13 @@ __global__ __launch_bounds__(64 * WAVES) void paged_attn_kernel(const PagedAttnA
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (the wave's other lanes read them)
       return __ballot(ok);
     };
-    auto logits = [&](int i) -> float* {  // of the wave's i-th tile
-      if (!a.sums || r >= heads) return nullptr;
+    auto logits = [&](int i) {  // of the wave's i-th tile
       const int at = v0 + (wave + WAVES * i) * kTile;
-      return a.logits + (((int64_t(hkv) * a.c.B + b) * a.max_units + at / kPagedUnit) * a.G + h0 + r) * kPagedUnit + at % kPagedUnit +
-             8 * j;
+      return [=, &a](int x) -> float* {
+        const int h = h0 + 16 * x + r;
+        if (!a.sums || h >= a.G) return nullptr;
+        return a.logits + (((int64_t(hkv) * a.c.B + b) * a.max_units + at / kPagedUnit) * a.G + h) * kPagedUnit + at % kPagedUnit + 8 * j;
+      };
     };
     auto walk = [&](auto mode) {
       constexpr bool ONCE = decltype(mode)::value;
@@ -502,57 +516,61 @@ __global__ __launch_bounds__(64 * WAVES) void paged_attn_kernel(const PagedAttnA
       if (once) walk(Yes{});
       else walk(No{});
     }
-    __syncthreads();
 
-    // the four waves' results, in wave order
-    const float l = quarters_sum(w.l);
-    if (j == 0) {
-      sh.m[wave][r] = w.m;
-      sh.l[wave][r] = l;
-    }
+    // the waves' results, in wave order
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int x = 0; x < RT; ++x) {
+      __syncthreads();
+      const float l = quarters_sum(w.l[x]);
+      if (j == 0) {
+        sh.m[wave][r] = w.m[x];
+        sh.l[wave][r] = l;
+      }
 #pragma unroll
-      for (int c = 0; c < NC; ++c) sh.o[wave][r][(4 * j + i) * NC + c] = w.acc[c][i];
-    __syncthreads();
-    const int oh = tid >> 4, od = (tid & 15) * NC;  // this thread's head and dims
-    float m = kNegInf;
+      for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int x = 0; x < WAVES; ++x) m = fmaxf(m, sh.m[x][oh]);
-    const float ref = m == kNegInf ? 0.f : m;
-    float sum = 0.f, o[NC] = {};
+        for (int c = 0; c < NC; ++c) sh.o[wave][r][(4 * j + i) * NC + c] = w.acc[x][c][i];
+      __syncthreads();
+      for (int y = tid; y < 256; y += 64 * WAVES) {
+        const int oh = y >> 4, od = (y & 15) * NC, h = h0 + 16 * x + oh;  // this thread's head and dims
+        if (h >= a.G) continue;
+        float m = kNegInf;
 #pragma unroll
-    for (int x = 0; x < WAVES; ++x) {
-      const float f = fast_exp2(sh.m[x][oh] - ref);
-      sum += f * sh.l[x][oh];
+        for (int v = 0; v < WAVES; ++v) m = fmaxf(m, sh.m[v][oh]);
+        const float ref = m == kNegInf ? 0.f : m;
+        float sum = 0.f, o[NC] = {};
 #pragma unroll
-      for (int c = 0; c < NC; ++c) o[c] += f * sh.o[x][oh][od + c];
-    }
-    if (oh < heads) {  // (with 8 waves, the first 4)
-      const int hq = hkv * a.G + h0 + oh;
-      if (whole) {
-        float ls = sum, scale = 1.f;
-        if (a.sinks) {
-          const float sink = a.sinks[hq] * kLog2e, top = fmaxf(m, sink);
-          if (top != kNegInf) {
-            scale = fast_exp2(ref - top);
-            ls = (m == kNegInf ? 0.f : sum * scale) + fast_exp2(sink - top);
-            m = top;
-          }
+        for (int v = 0; v < WAVES; ++v) {
+          const float f = fast_exp2(sh.m[v][oh] - ref);
+          sum += f * sh.l[v][oh];
+#pragma unroll
+          for (int c = 0; c < NC; ++c) o[c] += f * sh.o[v][oh][od + c];
         }
-        const float inv = ls == 0.f || sum == 0.f ? 0.f : scale * a.oscale / ls;
+        const int hq = hkv * a.G + h;
+        if (whole) {
+          float ls = sum, scale = 1.f;
+          if (a.sinks) {
+            const float sink = a.sinks[hq] * kLog2e, top = fmaxf(m, sink);
+            if (top != kNegInf) {
+              scale = fast_exp2(ref - top);
+              ls = (m == kNegInf ? 0.f : sum * scale) + fast_exp2(sink - top);
+              m = top;
+            }
+          }
+          const float inv = ls == 0.f || sum == 0.f ? 0.f : scale * a.oscale / ls;
 #pragma unroll
-        for (int c = 0; c < NC; ++c) o[c] = sum == 0.f ? 0.f : o[c] * inv;
-        store_out<E, NC>(a.o + int64_t(b) * a.so[0] + int64_t(hq) * a.so[1] + od * E::EB, o);
-        if (a.sums && (tid & 15) == 0) a.lse[int64_t(b) * a.Hq + hq] = (m == kNegInf ? 0.f : m) + fast_log2(ls);
-      } else {
-        const int64_t slot = int64_t(stream) * a.parts * 2 + part_slot(part, per, start);
-        float* po = a.part_o + (slot * 16 + oh) * D + od;
+          for (int c = 0; c < NC; ++c) o[c] = sum == 0.f ? 0.f : o[c] * inv;
+          store_out<E, NC>(a.o + int64_t(b) * a.so[0] + int64_t(hq) * a.so[1] + od * E::EB, o);
+          if (a.sums && (y & 15) == 0) a.lse[int64_t(b) * a.Hq + hq] = (m == kNegInf ? 0.f : m) + fast_log2(ls);
+        } else {
+          const int64_t slot = (int64_t(hkv) * a.row_tiles + h / 16) * a.parts * 2 + part_slot(part, per, start);
+          float* po = a.part_o + (slot * 16 + oh) * D + od;
 #pragma unroll
-        for (int c = 0; c < NC; ++c) po[c] = o[c];
-        if ((tid & 15) == 0) {
-          a.part_ml[slot * 32 + oh] = m;
-          a.part_ml[slot * 32 + 16 + oh] = sum;
+          for (int c = 0; c < NC; ++c) po[c] = o[c];
+          if ((y & 15) == 0) {
+            a.part_ml[slot * 32 + oh] = m;
+            a.part_ml[slot * 32 + 16 + oh] = sum;
+          }
         }
       }
     }
@@ -699,14 +717,19 @@ __global__ __launch_bounds__(kThreads) void paged_finish_kernel(const PagedAttnA
 
 template <typename E, int D>
 hipError_t run(const PagedAttnArgs& a, hipStream_t s) {
-  const unsigned streams = unsigned(a.c.Hkv * a.row_tiles), B = unsigned(a.c.B);
-  const dim3 grid(streams * (a.parts ? unsigned(a.parts) : B));
-  // 8 waves where the workgroups are few and the waves' tables and tiles fit the 64 KB of LDS
-  if constexpr (sizeof(Shared<E, D, 8>) <= 65536) {
-    if (!a.wide) hipLaunchKernelGGL((paged_attn_kernel<E, D, 4>), grid, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((paged_attn_kernel<E, D, 8>), grid, dim3(512), 0, s, a);
+  const unsigned B = unsigned(a.c.B), parts = a.parts ? unsigned(a.parts) : B;
+  const unsigned streams = unsigned(a.c.Hkv) * unsigned((a.row_tiles + a.rt - 1) / a.rt);
+  const auto launch = [&](auto kernel, int waves) { hipLaunchKernelGGL(kernel, dim3(streams * parts), dim3(64 * waves), 0, s, a); };
+  constexpr bool EIGHT = sizeof(Shared<E, D, 8>) <= 65536;  // (the waves' tables and tiles in LDS)
+  const int waves = a.rt == 2 || (a.waves == 8 && !EIGHT) ? 4 : a.waves;
+  if (a.rt == 2) {
+    if constexpr (paged_pairs(D, E::CB)) launch(paged_attn_kernel<E, D, 4, 2>, 4);
+  } else if (waves == 8) {
+    if constexpr (EIGHT) launch(paged_attn_kernel<E, D, 8, 1>, 8);
+  } else if (waves == 1) {
+    launch(paged_attn_kernel<E, D, 1, 1>, 1);
   } else {
-    hipLaunchKernelGGL((paged_attn_kernel<E, D, 4>), grid, dim3(256), 0, s, a);
+    launch(paged_attn_kernel<E, D, 4, 1>, 4);
   }
   const hipError_t e = hipGetLastError();
   const unsigned joins = a.parts ? unsigned(a.Hq) * B : 0u;
