@@ -111,6 +111,11 @@ ATTEND = [
     ("bf16", "bf16", 32, 6, 2, 16, "hnd", (70, 1, 800), None, 0, True),
     ("bf16", "bf16", 16, 5, 1, 16, "nhd", (70, 1, 800), 100, 2, False),
     ("bf16", "bf16", 64, 33, 1, 16, "hnd", (70, 1, 800), None, 0, True),
+    ("bf16", "bf16", 64, 64, 1, 16, "nhd", (1100, 1, 0, 700), None, 0, True),
+    ("bf16", "bf16", 128, 40, 1, 16, "hnd", (1100, 5), None, 0, False),
+    ("fp16", "fp8", 128, 34, 1, 16, "hnd", (1030, 5), None, 0, True),
+    ("bf16", "bf16", 64, 8, 2, 16, "hnd", (1025, 2000, 31, 0, 1500), None, 0, False),
+    ("bf16", "bf16", 128, 4, 2, 16, "nhd", (1500, 2, 1024), 1200, 7, True),
     ("fp16", "fp16", 64, 8, 8, 16, "hnd", (70, 1, 800, 129), None, 0, False),
     ("fp16", "fp16", 16, 4, 1, 1, "hnd", (70, 1, 600), None, 0, False),
     ("fp16", "fp16", 128, 20, 1, 256, "hnd", (300, 1, 600), None, 0, True),
@@ -148,6 +153,84 @@ def test_attention(fa, gpu, case, sums):
         err = (w.double().cpu() - ref_sums).abs()
         assert bool((err <= tol).all()), float((err - tol).max())
         assert torch.equal(w.cpu()[add == 0], w0[add == 0])  # keys that nobody sees keep their sums
+
+
+@pytest.mark.parametrize("B,Hq,Hkv,D,cache,W", [(520, 4, 2, 64, "bf16", 128), (600, 2, 2, 16, "fp16", 33), (513, 2, 2, 64, "fp8", 40),
+                                                (140, 4, 2, 64, "bf16", 150), (90, 3, 3, 128, "bf16", None), (64, 2, 2, 64, "bf16", None)])
+def test_many_short_sequences(fa, gpu, B, Hq, Hkv, D, cache, W):
+    """Batches large enough for a wave, or a workgroup of four, a sequence."""
+    dtype = "fp16" if cache == "fp16" else "bf16"
+    g = torch.Generator().manual_seed(B)
+    lens = torch.randint(0, 260, (B,), generator=g).tolist()
+    c = make(B, dtype, cache, D, Hq, Hkv, 16, "hnd", lens, extra=100 if B == 64 else 0)
+    ref, mag, _ = oracle.attention(c["q"], c["kp"], c["vp"], c["table"], c["lens"], W, 3 if W else 0, c["sinks"], descale=c["descale"])
+    o = fa.paged_attention(c["q"].to(gpu), c["kp"].to(gpu), c["vp"].to(gpu), c["table"].to(gpu), c["lens"].to(gpu), W, 3 if W else 0,
+                           c["sinks"].to(gpu), descale=c["descale"])
+    check_attention(o, c, ref, mag, dtype, D, 260, 1 / math.sqrt(D), W, 3 if W else 0)
+
+
+def test_large_cache(fa, gpu):
+    """270 MB of K and V, so that loads are marked as read once, in two layouts, with weights."""
+    B, Hq, Hkv, D, page = 3, 16, 2, 64, 64
+    lens = [300001, 70000, 140000]
+    g = torch.Generator(device=gpu).manual_seed(5)
+    used = [-(-n // page) for n in lens]
+    P = sum(used)
+    order = torch.randperm(P, generator=g, device=gpu).to(torch.int32)
+    table = torch.full((B, max(used)), -1, dtype=torch.int32, device=gpu)
+    for b in range(B):
+        table[b, :used[b]] = order[sum(used[:b]):sum(used[:b + 1])]
+    q = torch.randn(B, Hq, D, generator=g, device=gpu).to(torch.bfloat16) * 2
+    tl = torch.tensor(lens, dtype=torch.int32, device=gpu)
+    for layout in ("hnd", "nhd"):
+        shape = (P, Hkv, page, D) if layout == "hnd" else (P, page, Hkv, D)
+        kp, vp = (torch.randn(shape, generator=g, device=gpu).to(torch.bfloat16) for _ in range(2))
+        if layout == "nhd":
+            kp, vp = kp.transpose(1, 2), vp.transpose(1, 2)
+        sums = torch.zeros(B, Hkv, max(used) * page, device=gpu)
+        o = fa.paged_attention(q, kp, vp, table, tl, weight_sums=sums)
+        for b, n in enumerate(lens):
+            at = table[b, :used[b]].long()
+            for h in range(Hkv):
+                k, v = (x[at, h].reshape(-1, D)[:n].double() for x in (kp, vp))
+                p = torch.softmax(q[b, 8 * h:8 * h + 8].double() @ k.t() / 8, -1)
+                ref, mag = p @ v, p @ v.abs()
+                a = float((q[b, 8 * h:8 * h + 8].double().abs() @ k.abs().t()).max()) / 8
+                d = 2 * (D + 4) * 2.0 ** -24 * a + 2.0 ** -21
+                tol = (d + 2.0 ** -17 + n * 2.0 ** -24) * mag + 2.0 ** -8 * ref.abs()
+                err = (o[b, 8 * h:8 * h + 8].double() - ref).abs()
+                assert bool((err <= tol).all()), (layout, b, h, float((err - tol).max()))
+                w = p.sum(0)
+                assert bool(((sums[b, h, :n].double() - w).abs() <= (d + n * 2.0 ** -24) * w + 2.0 ** -23 * w).all())
+            assert not sums[b, :, n:].any()
+
+
+def test_offsets_past_32_bits(fa, gpu):
+    """Pages 4 GiB apart: a pool of all layers, of which this is one layer's view."""
+    P, Hkv, page, D = 3, 2, 16, 64
+    step = 2 ** 31  # elements
+    pools = [torch.empty(2 * step + Hkv * page * D, dtype=torch.bfloat16, device=gpu).as_strided((P, Hkv, page, D), (step, page * D, D, 1))
+             for _ in range(2)]
+    small = [torch.randn(P, Hkv, page, D, generator=torch.Generator().manual_seed(i)).to(torch.bfloat16) for i in range(2)]
+    for x, y in zip(pools, small):
+        x.copy_(y)
+    table = torch.tensor([[2, 1]], dtype=torch.int32)
+    lens = torch.tensor([21], dtype=torch.int32)
+    g = torch.Generator().manual_seed(9)
+    k, v = (torch.randn(1, Hkv, D, generator=g).to(torch.bfloat16) for _ in range(2))
+    q = torch.randn(1, 4, D, generator=g).to(torch.bfloat16)
+    fa.paged_append(k.to(gpu), v.to(gpu), *pools, table.to(gpu), lens.to(gpu))
+    small = oracle.append(k, v, *small, table, lens)
+    o = fa.paged_attention(q.to(gpu), *pools, table.to(gpu), lens.to(gpu))
+    ref, mag, _ = oracle.attention(q, *small, table, lens)
+    check_attention(o, dict(q=q, kp=small[0], vp=small[1], table=table, lens=lens, descale=(1, 1)), ref, mag, "bf16", D, 21, 0.125)
+    sums = torch.rand(1, Hkv, 32, generator=g)
+    new_table = torch.tensor([[0]], dtype=torch.int32)
+    want = oracle.evict(*small, table, lens, sums, 12, new_table, 1, 2)
+    left, new = fa.paged_evict(*pools, table.to(gpu), lens.to(gpu), sums.to(gpu), 12, new_table.to(gpu), 1, 2)
+    same(new, want[3])
+    same(pools[0].contiguous(), want[0])
+    same(pools[1].contiguous(), want[1])
 
 
 @pytest.mark.parametrize("scale", [0.0, -0.3, 2.0])
