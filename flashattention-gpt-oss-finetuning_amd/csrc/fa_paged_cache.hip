@@ -132,9 +132,7 @@ __device__ __forceinline__ uint32_t with_digit(uint32_t prefix, uint32_t d, int 
 
 constexpr int kSelectWaves = kSelectThreads / 64;
 
-constexpr int kSelectMost = 16;  // entries that a thread has in registers, at most
-
-// A chunk's entries in registers: entry first + 1024 e + tid is x[e], u[e] its place in the order.
+// A thread's entries of a chunk, in registers: entry first + EACH tid + e is x[e], u[e] its place in the order.
 template <int EACH>
 struct Entries {
   float x[EACH];
@@ -145,25 +143,35 @@ struct Entries {
 struct SelectShared {
   uint32_t hist[kBins];
   int wave[2][kSelectWaves];
-  uint32_t runs[kSelectMost * kSelectWaves];
   uint32_t digit;
   int need, prior, equal;
 };
 
+// The chunk's weights.  `width` of them are in memory, whatever n is, so these loads do not wait for lens.
 template <int EACH>
-__device__ __forceinline__ void read_entries(Entries<EACH>& t, const float* x, int first, int n, int lo, int hi) {
-  const int tid = threadIdx.x;
+__device__ __forceinline__ void read_entries(Entries<EACH>& t, const float* x, int first, int width) {
+  typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));  // (rows start where the caller's strides put them)
+  const int i0 = first + EACH * int(threadIdx.x);
+  if (i0 + EACH <= width) {
 #pragma unroll
-  for (int e = 0; e < EACH; ++e) {
-    const int i = first + e * kSelectThreads + tid;
-    t.x[e] = i < n ? x[i] : 0.f;
+    for (int e = 0; e < EACH; e += 4) {
+      const f32x4 v = *reinterpret_cast<const f32x4_any*>(x + i0 + e);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) t.x[e + c] = v[c];
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) t.x[e] = i0 + e < width ? x[i0 + e] : 0.f;
   }
+}
+template <int EACH>
+__device__ __forceinline__ void order_entries(Entries<EACH>& t, int first, int lo, int hi) {
+  const int i0 = first + EACH * int(threadIdx.x);
   t.open = 0;
 #pragma unroll
   for (int e = 0; e < EACH; ++e) {
-    const int i = first + e * kSelectThreads + tid;
     t.u[e] = order_of(t.x[e]);
-    t.open |= uint32_t(i >= lo && i < hi) << e;
+    t.open |= uint32_t(i0 + e >= lo && i0 + e < hi) << e;
   }
 }
 
@@ -178,33 +186,32 @@ __device__ __forceinline__ void count_digits(SelectShared& sh, const Entries<EAC
   __syncthreads();
 }
 
-// cnt: entries in this thread's bins 2047 - 2 tid and 2046 - 2 tid; old: those of earlier chunks.  Finds the bin of the
-// need-th entry from the largest: its digit; need becomes the number of its entries that stay; prior grows by the
-// entries of earlier chunks in larger bins; equal: theirs in this bin.
-__device__ __forceinline__ uint32_t find_digit(SelectShared& sh, const int (&cnt)[2], const int (&old)[2], int& need, int& prior, int& equal) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int both = cnt[0] + cnt[1], both_old = old[0] + old[1];
-  int x = both, y = both_old;
+// The sum over the workgroup's threads before this one, by one of two LDS rows.  A barrier is inside; the caller has one before the
+// row is used again.
+__device__ __forceinline__ int sum_before(SelectShared& sh, int row, int x) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int y = x;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
-    const int p = __shfl_up(x, o), q = __shfl_up(y, o);
-    if (lane >= o) {
-      x += p;
-      y += q;
-    }
+    const int p = __shfl_up(y, o);
+    if (lane >= o) y += p;
   }
-  if (lane == 63) {
-    sh.wave[0][wave] = x;
-    sh.wave[1][wave] = y;
-  }
+  if (lane == 63) sh.wave[row][wave] = y;
   __syncthreads();
-  int before = x - both, before_old = y - both_old;
+  int before = y - x;
 #pragma unroll
-  for (int w = 0; w < kSelectWaves; ++w) {
-    before += w < wave ? sh.wave[0][w] : 0;
-    before_old += w < wave ? sh.wave[1][w] : 0;
-  }
-  if (before < need && before + both >= need) {  // (one thread: 1 <= need <= all entries)
+  for (int w = 0; w < kSelectWaves; ++w) before += w < wave ? sh.wave[row][w] : 0;
+  return before;
+}
+
+// cnt: entries in this thread's bins 2047 - 2 tid and 2046 - 2 tid; old: those of earlier chunks (MANY).  Finds the bin of
+// the need-th entry from the largest: its digit; need becomes the number of its entries that stay; prior grows by the
+// entries of earlier chunks in larger bins; equal: theirs in this bin.
+template <bool MANY>
+__device__ __forceinline__ uint32_t find_digit(SelectShared& sh, const int (&cnt)[2], const int (&old)[2], int& need, int& prior, int& equal) {
+  const int tid = threadIdx.x;
+  const int before = sum_before(sh, 0, cnt[0] + cnt[1]), before_old = MANY ? sum_before(sh, 1, old[0] + old[1]) : 0;
+  if (before < need && before + cnt[0] + cnt[1] >= need) {  // (one thread: 1 <= need <= all entries)
     const int i = before + cnt[0] >= need ? 0 : 1;
     sh.digit = uint32_t(kBins - 1 - 2 * tid - i);
     sh.need = need - before - (i ? cnt[0] : 0);
@@ -213,8 +220,10 @@ __device__ __forceinline__ uint32_t find_digit(SelectShared& sh, const int (&cnt
   }
   __syncthreads();
   need = sh.need;
-  prior += sh.prior;
-  equal = sh.equal;
+  if (MANY) {
+    prior += sh.prior;
+    equal = sh.equal;
+  }
   return sh.digit;
 }
 
@@ -222,53 +231,32 @@ __device__ __forceinline__ uint32_t find_digit(SelectShared& sh, const int (&cnt
 // of those equal to it the first `need` (equal of which are in earlier chunks).  rank: entries of earlier chunks that
 // stay for another reason.
 template <int EACH>
-__device__ __forceinline__ void write_kept(SelectShared& sh, const Entries<EACH>& t, int first, int n, int m, uint32_t least, int need, int rank, int equal,
-                                           int* kept, float* y) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const unsigned long long below = (1ull << lane) - 1;
-  uint32_t mine[EACH];  // entries of this wave's row e before this lane: those that stay, and << 16 the equal ones
+__device__ __forceinline__ void write_kept(SelectShared& sh, const Entries<EACH>& t, int first, int n, int m, uint32_t least, int need, int rank,
+                                           int equal, int* kept, float* y) {
+  const int i0 = first + EACH * int(threadIdx.x);
   uint32_t stays = 0, equals = 0;
 #pragma unroll
   for (int e = 0; e < EACH; ++e) {
-    const bool open = t.open >> e & 1, have = first + e * kSelectThreads + tid < n;
-    const bool s = have && (!open || t.u[e] > least), q = open && t.u[e] == least;
-    const unsigned long long ms = __ballot(s), mq = __ballot(q);
-    mine[e] = uint32_t(__popcll(ms & below)) | uint32_t(__popcll(mq & below)) << 16;
-    stays |= uint32_t(s) << e;
-    equals |= uint32_t(q) << e;
-    if (lane == 0) sh.runs[e * kSelectWaves + wave] = uint32_t(__popcll(ms)) | uint32_t(__popcll(mq)) << 16;
+    const bool open = t.open >> e & 1;
+    stays |= uint32_t(i0 + e < n && (!open || t.u[e] > least)) << e;
+    equals |= uint32_t(open && t.u[e] == least) << e;
   }
-  __syncthreads();
-  if (wave == 0) {  // exclusive sums over the runs, in order (both halves stay below 2^16: a chunk has 2^14 entries)
-    constexpr int PER = EACH * kSelectWaves / 64;  // (EACH is a multiple of 4)
-    uint32_t c[PER], all = 0;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) all += c[i] = sh.runs[lane * PER + i];
-    uint32_t x = all;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const uint32_t p = uint32_t(__shfl_up(int(x), o));
-      if (lane >= o) x += p;
-    }
-    x -= all;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      sh.runs[lane * PER + i] = x;
-      x += c[i];
-    }
-  }
-  __syncthreads();
+  // (both halves of the sums stay below 2^16: a chunk has at most 2^14 entries)
+  const int before = sum_before(sh, 0, __popc(stays) | __popc(equals) << 16);
+  rank += before & 0xffff;
+  equal += before >> 16;
 #pragma unroll
   for (int e = 0; e < EACH; ++e) {
-    const uint32_t x = sh.runs[e * kSelectWaves + wave] + mine[e];
-    const int before = equal + int(x >> 16);  // equal entries before this one
-    if ((stays >> e & 1) || ((equals >> e & 1) && before < need)) {
-      const int r = rank + int(x & 0xffff) + imin(before, need);
+    const bool s = stays >> e & 1, q = equals >> e & 1;
+    if (s || (q && equal < need)) {
+      const int r = rank + imin(equal, need);
       if (unsigned(r) < unsigned(m)) {  // (always, unless the weights change under the running call)
-        kept[r] = first + e * kSelectThreads + tid;
+        kept[r] = i0 + e;
         y[r] = t.x[e];
       }
     }
+    rank += s;
+    equal += q;
   }
 }
 
@@ -281,9 +269,11 @@ __global__ __launch_bounds__(kSelectThreads) void paged_select_kernel(const Evic
   constexpr int kChunk = EACH * kSelectThreads;
   __shared__ SelectShared sh;
   const int chunk = blockIdx.x % a.chunks, row = blockIdx.x / a.chunks, hkv = row % a.c.Hkv, b = row / a.c.Hkv;
-  const int tid = threadIdx.x;
-  const int n = seq_len(a.c, b), m = imin(n, a.keep), first = chunk * kChunk;
+  const int tid = threadIdx.x, first = chunk * kChunk;
   const bool last = a.chunks == 1 || stage == kDigits;
+  Entries<EACH> t;
+  read_entries(t, a.sums + int64_t(b) * a.ssum[0] + int64_t(hkv) * a.ssum[1], first, a.sums_width);
+  const int n = seq_len(a.c, b), m = imin(n, a.keep);
   float* y = a.new_sums + int64_t(b) * a.snew[0] + int64_t(hkv) * a.snew[1];
   if (last) {
     if (hkv == 0 && chunk == 0 && tid == 0) a.new_lens[b] = m;
@@ -294,50 +284,47 @@ __global__ __launch_bounds__(kSelectThreads) void paged_select_kernel(const Evic
   const int choose = n > a.keep ? a.keep - a.S - a.R : 0;
   if (first >= n || (choose == 0 && !last)) return;
   const int lo = n > a.keep ? a.S : 0, hi = n > a.keep ? n - a.R : 0;
-  Entries<EACH> t;
-  read_entries(t, a.sums + int64_t(b) * a.ssum[0] + int64_t(hkv) * a.ssum[1], first, n, lo, hi);
   uint32_t prefix = choose > 0 ? 0u : 0xffffffffu;  // (nothing to choose: no number is above, and none equal is needed)
   int need = choose, prior = 0, equal = 0;
+  if (choose > 0 && a.chunks > 1 && stage > 0) {
+    const int chunks = (n + kChunk - 1) / kChunk;
+    int* state = a.state + (int64_t(row) * a.chunks + chunk) * 3;  // this workgroup's prefix, need and prior
+    if (stage > 1) {
+      prefix = uint32_t(state[0]);
+      need = state[1];
+      prior = state[2];
+    }
+    const uint32_t* of = reinterpret_cast<const uint32_t*>(a.counts + (int64_t(row) * kDigits + stage - 1) * a.chunks * kBins) + tid;
+    int cnt[2] = {0, 0}, old[2] = {0, 0};
+#pragma unroll 8
+    for (int c = 0; c < chunks; ++c) {
+      const uint32_t x = of[c * (kBins / 2)];
+      if (c == chunk) {
+        old[0] = cnt[0];
+        old[1] = cnt[1];
+      }
+      cnt[0] += int(x & 0xffff);
+      cnt[1] += int(x >> 16);
+    }
+    prefix = with_digit(prefix, find_digit<true>(sh, cnt, old, need, prior, equal), stage - 1);
+    if (!last && tid == 0) {
+      state[0] = int(prefix);
+      state[1] = need;
+      state[2] = prior;
+    }
+  }
+  order_entries(t, first, lo, hi);
+  if (!last) {  // counts: [digit][chunk][2047 - value]
+    count_digits(sh, t, prefix, stage);
+    reinterpret_cast<uint32_t*>(a.counts + ((int64_t(row) * kDigits + stage) * a.chunks + chunk) * kBins)[tid] =
+        sh.hist[kBins - 1 - 2 * tid] | sh.hist[kBins - 2 - 2 * tid] << 16;
+    return;
+  }
   if (choose > 0 && a.chunks == 1) {
     for (int q = 0; q < kDigits; ++q) {
       count_digits(sh, t, prefix, q);
       const int cnt[2] = {int(sh.hist[kBins - 1 - 2 * tid]), int(sh.hist[kBins - 2 - 2 * tid])}, old[2] = {0, 0};
-      prefix = with_digit(prefix, find_digit(sh, cnt, old, need, prior, equal), q);
-    }
-  } else if (choose > 0) {
-    const int chunks = (n + kChunk - 1) / kChunk;
-    int* state = a.state + (int64_t(row) * a.chunks + chunk) * 3;  // this workgroup's prefix, need and prior
-    uint16_t* counts = a.counts + int64_t(row) * kDigits * a.chunks * kBins;  // [digit][chunk][2047 - value]
-    if (stage > 0) {
-      if (stage > 1) {
-        prefix = uint32_t(state[0]);
-        need = state[1];
-        prior = state[2];
-      }
-      const uint32_t* of = reinterpret_cast<const uint32_t*>(counts + int64_t(stage - 1) * a.chunks * kBins) + tid;
-      int cnt[2] = {0, 0}, old[2] = {0, 0};
-#pragma unroll 8
-      for (int c = 0; c < chunks; ++c) {
-        const uint32_t x = of[c * (kBins / 2)];
-        if (c == chunk) {
-          old[0] = cnt[0];
-          old[1] = cnt[1];
-        }
-        cnt[0] += int(x & 0xffff);
-        cnt[1] += int(x >> 16);
-      }
-      prefix = with_digit(prefix, find_digit(sh, cnt, old, need, prior, equal), stage - 1);
-      if (!last && tid == 0) {
-        state[0] = int(prefix);
-        state[1] = need;
-        state[2] = prior;
-      }
-    }
-    if (!last) {
-      count_digits(sh, t, prefix, stage);
-      reinterpret_cast<uint32_t*>(counts + (int64_t(stage) * a.chunks + chunk) * kBins)[tid] =
-          sh.hist[kBins - 1 - 2 * tid] | sh.hist[kBins - 2 - 2 * tid] << 16;
-      return;
+      prefix = with_digit(prefix, find_digit<false>(sh, cnt, old, need, prior, equal), q);
     }
   }
   const int fixed = n > a.keep ? imin(first, lo) + imax(0, first - hi) : first;  // entries of earlier chunks that stay by their place
