@@ -599,9 +599,9 @@ __device__ __forceinline__ Pieces pieces_of(const PagedAttnArgs& a, int b) {
 
 // Query head hq of sequence b, if it was cut: its pieces' results.  D / 4 threads take a piece; every thread adds its
 // pieces in order, then the groups of threads are added in order.
-template <typename E, int D>
+template <typename E, int D, int THREADS>
 __device__ __forceinline__ void join_head(const PagedAttnArgs& a, int b, int hq, float* smem) {
-  constexpr int T = D / 4, GROUPS = kThreads / T;
+  constexpr int T = D / 4, GROUPS = THREADS / T;
   const Pieces ps = pieces_of(a, b);
   if (ps.first >= ps.last) return;
   const int hkv = hq / a.G, h = hq % a.G, oh = h % 16;
@@ -627,16 +627,16 @@ __device__ __forceinline__ void join_head(const PagedAttnArgs& a, int b, int hq,
   for (int i = 0; i < 4; ++i) smem[group * D + d + i] = o[i];
   if (d == 0) smem[GROUPS * D + group] = sum;
   __syncthreads();
-  if (tid < D) {
+  for (int i = tid; i < D; i += THREADS) {
     float x = 0.f, s = 0.f;
 #pragma unroll 8
     for (int g = 0; g < GROUPS; ++g) {
-      x += smem[g * D + tid];
+      x += smem[g * D + i];
       s += smem[GROUPS * D + g];
     }
     const float ls = s + (sink == kNegInf ? 0.f : fast_exp2(sink - ref));
     const float out[1] = {s == 0.f ? 0.f : x * (a.oscale / ls)};
-    store_out<E, 1>(a.o + int64_t(b) * a.so[0] + int64_t(hq) * a.so[1] + tid * E::EB, out);
+    store_out<E, 1>(a.o + int64_t(b) * a.so[0] + int64_t(hq) * a.so[1] + i * E::EB, out);
   }
 }
 
@@ -704,15 +704,17 @@ __device__ __forceinline__ void add_weights(const PagedAttnArgs& a, int b, int h
 }
 
 // Workgroups [0, joins) join heads, the ones behind them add weights.
-template <typename E, int D>
-__global__ __launch_bounds__(kThreads) void paged_finish_kernel(const PagedAttnArgs a, unsigned joins) {
-  __shared__ float smem[kThreads * 4 + 64];
+template <typename E, int D, int THREADS>
+__global__ __launch_bounds__(THREADS) void paged_finish_kernel(const PagedAttnArgs a, unsigned joins) {
+  __shared__ float smem[THREADS * 4 + 64];
   if (blockIdx.x < joins) {
-    join_head<E, D>(a, blockIdx.x / a.Hq, blockIdx.x % a.Hq, smem);
+    join_head<E, D, THREADS>(a, blockIdx.x / a.Hq, blockIdx.x % a.Hq, smem);
     return;
   }
-  const unsigned i = blockIdx.x - joins, chunks = unsigned((a.max_units * kPagedUnit + kSumKeys - 1) / kSumKeys);
-  add_weights(a, int(i / chunks / unsigned(a.c.Hkv)), int(i / chunks % unsigned(a.c.Hkv)), int(i % chunks), smem);
+  if constexpr (THREADS == kThreads) {
+    const unsigned i = blockIdx.x - joins, chunks = unsigned((a.max_units * kPagedUnit + kSumKeys - 1) / kSumKeys);
+    add_weights(a, int(i / chunks / unsigned(a.c.Hkv)), int(i / chunks % unsigned(a.c.Hkv)), int(i % chunks), smem);
+  }
 }
 
 template <typename E, int D>
@@ -735,7 +737,9 @@ hipError_t run(const PagedAttnArgs& a, hipStream_t s) {
   const unsigned joins = a.parts ? unsigned(a.Hq) * B : 0u;
   const unsigned adds = a.sums ? unsigned((a.max_units * kPagedUnit + kSumKeys - 1) / kSumKeys) * unsigned(a.c.Hkv) * B : 0u;
   if (e != hipSuccess || joins + adds == 0) return e;
-  hipLaunchKernelGGL((paged_finish_kernel<E, D>), dim3(joins + adds), dim3(kThreads), 0, s, a, joins);
+  // a wave a head where the sequences have few pieces each
+  if (adds == 0 && a.parts <= 4 * a.c.B) hipLaunchKernelGGL((paged_finish_kernel<E, D, 64>), dim3(joins), dim3(64), 0, s, a, joins);
+  else hipLaunchKernelGGL((paged_finish_kernel<E, D, kThreads>), dim3(joins + adds), dim3(kThreads), 0, s, a, joins);
   return hipGetLastError();
 }
 

@@ -156,13 +156,14 @@ def test_attention(fa, gpu, case, sums):
 
 
 @pytest.mark.parametrize("B,Hq,Hkv,D,cache,W", [(520, 4, 2, 64, "bf16", 128), (600, 2, 2, 16, "fp16", 33), (513, 2, 2, 64, "fp8", 40),
-                                                (140, 4, 2, 64, "bf16", 150), (90, 3, 3, 128, "bf16", None), (64, 2, 2, 64, "bf16", None)])
+                                                (140, 4, 2, 64, "bf16", 150), (90, 3, 3, 128, "bf16", None), (64, 2, 2, 64, "bf16", None),
+                                                (70, 2, 2, 64, "bf16", None), (70, 4, 4, 128, "fp8", None)])
 def test_many_short_sequences(fa, gpu, B, Hq, Hkv, D, cache, W):
     """Batches large enough for a wave, or a workgroup of four, a sequence."""
     dtype = "fp16" if cache == "fp16" else "bf16"
     g = torch.Generator().manual_seed(B)
     lens = torch.randint(0, 260, (B,), generator=g).tolist()
-    c = make(B, dtype, cache, D, Hq, Hkv, 16, "hnd", lens, extra=100 if B == 64 else 0)
+    c = make(B, dtype, cache, D, Hq, Hkv, 16, "hnd", lens, extra={64: 100, 70: 150}.get(B, 0))
     ref, mag, _ = oracle.attention(c["q"], c["kp"], c["vp"], c["table"], c["lens"], W, 3 if W else 0, c["sinks"], descale=c["descale"])
     o = fa.paged_attention(c["q"].to(gpu), c["kp"].to(gpu), c["vp"].to(gpu), c["table"].to(gpu), c["lens"].to(gpu), W, 3 if W else 0,
                            c["sinks"].to(gpu), descale=c["descale"])
