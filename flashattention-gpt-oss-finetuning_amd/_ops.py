@@ -552,6 +552,13 @@ def _check_sums(sums, k_pages, B):
                          f"{list(sums.shape)}")
 
 
+def _distinct(**tensors):
+    """Entries that share memory cannot be written."""
+    for name, t in tensors.items():
+        if any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape)):
+            raise ValueError(f"{name} is written in place: its entries must not share memory (an expanded tensor)")
+
+
 def _changed(*tensors):
     """What a call wrote in place, as far as autograd's version counters go."""
     for t in tensors:
@@ -573,6 +580,7 @@ def paged_append(k, v, k_pages, v_pages, block_table, lens, cu, k_descale: float
         return b.paged_append(k, v, k_pages, v_pages, block_table, lens, cu, k_descale, v_descale)
     _refuse_traced("paged_append")
     c, held = _paged_cache(k_pages, v_pages, block_table, lens, k_descale, v_descale)
+    _distinct(k_pages=k_pages, v_pages=v_pages)
     k, v = _paged_input(k, k_pages, "k"), _paged_input(v, k_pages, "v")
     if k.shape[1] != k_pages.shape[1] or v.shape != k.shape or v.dtype != k.dtype:
         raise ValueError(f"k and v must both be [rows, Hkv, D] of one dtype, got {list(k.shape)} and {list(v.shape)}")
@@ -609,6 +617,7 @@ def paged_attention(q, k_pages, v_pages, block_table, lens, window: int, sink: i
     p.sinks = None if sk is None else sk.data_ptr()
     if weight_sums is not None:
         _check_sums(weight_sums, k_pages, B)
+        _distinct(weight_sums=weight_sums)
         p.weight_sums = weight_sums.data_ptr()
         p.sums_stride[:] = weight_sums.stride()[:2]
         p.sums_width = _i32(weight_sums.shape[2])
@@ -633,6 +642,7 @@ def paged_evict(k_pages, v_pages, block_table, lens, weight_sums, keep: int, new
     _refuse_traced("paged_evict")
     p = _lib.PagedEvictParams()
     p.cache, held = _paged_cache(k_pages, v_pages, block_table, lens, 1.0, 1.0)
+    _distinct(k_pages=k_pages, v_pages=v_pages)
     B, Hkv = p.cache.batch, p.cache.heads_kv
     _on_device(weight_sums, k_pages, "weight_sums", "k_pages")
     _on_device(new_table, k_pages, "new_table", "k_pages")

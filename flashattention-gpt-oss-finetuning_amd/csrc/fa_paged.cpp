@@ -80,8 +80,8 @@ constexpr int64_t kKeepBytes = int64_t(96) << 20;
 
 struct Plan {
   int max_units, row_tiles, rt, parts;
-  size_t part_o, part_ml, lse, logits;  // bytes
-  size_t bytes() const { return std::max<size_t>(256, part_o + part_ml + lse + logits); }
+  size_t starts, part_o, part_ml, lse, logits;  // bytes
+  size_t bytes() const { return std::max<size_t>(256, starts + part_o + part_ml + lse + logits); }
 };
 
 int plan(const fa_paged_attention_params* p, Plan* r) {
@@ -120,6 +120,7 @@ int plan(const fa_paged_attention_params* p, Plan* r) {
     if (!fa::grid_fits(streams * r->parts)) return FA_ERR_OVERFLOW;
   }
   const size_t slots = size_t(c.heads_kv) * r->row_tiles * r->parts * 2;
+  r->starts = r->parts ? align256((size_t(c.batch) + 1) * sizeof(int32_t)) : 0;
   r->part_o = align256(slots * 16 * c.head_dim * sizeof(float));
   r->part_ml = align256(slots * 32 * sizeof(float));
   r->lse = r->logits = 0;
@@ -228,10 +229,11 @@ int fa_paged_attention(const fa_paged_attention_params* p, void* workspace, size
   a.waves = r.parts ? 4 : wgs <= fa::device_cus() ? 8 : wgs >= kSingleWgs && r.max_units <= kSingleUnits ? 1 : 4;
   a.keep_units = int(std::min<int64_t>(kKeepBytes / (int64_t(fa::kPagedUnit) * 2 * c.head_dim * elem_bytes(c.dtype) * c.heads_kv), INT32_MAX));
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  a.part_o = reinterpret_cast<float*>(ws);
-  a.part_ml = reinterpret_cast<float*>(ws + r.part_o);
-  a.lse = reinterpret_cast<float*>(ws + r.part_o + r.part_ml);
-  a.logits = reinterpret_cast<float*>(ws + r.part_o + r.part_ml + r.lse);
+  a.starts = reinterpret_cast<int*>(ws);
+  a.part_o = reinterpret_cast<float*>(ws += r.starts);
+  a.part_ml = reinterpret_cast<float*>(ws += r.part_o);
+  a.lse = reinterpret_cast<float*>(ws += r.part_ml);
+  a.logits = reinterpret_cast<float*>(ws += r.lse);
   return status(fa::launch_paged_attention(a, p->dtype, c.dtype, c.head_dim, static_cast<hipStream_t>(stream)));
 }
 

@@ -53,6 +53,7 @@ struct PagedAttnArgs {
   int rt;                 // tiles of heads that a workgroup takes: 1, or 2 (paged_pairs)
   int keep_units;         // calls that read more units a KV head than this mark their loads as read once
   // workspace
+  int* starts;            // split calls: [B] the sequences' first units, and the units of a part
   float* part_o;          // [Hkv row_tiles][parts][2][16][D]
   float* part_ml;         // [Hkv row_tiles][parts][2][2][16]: maximum (log2 domain), sum
   float* lse;             // with sums: [B][Hq] (log2 domain), of the sequences that one workgroup took whole

@@ -55,16 +55,14 @@ __device__ __forceinline__ int units_of(const PagedAttnArgs& a, int b) {
   return b < a.c.B ? paged_units(visible(seq_len(a.c, b), a.W, a.S).count) : 0;
 }
 
-// Units of the sequences before b, and of all of them (every lane of the wave calls).
-__device__ __forceinline__ void units_before(const PagedAttnArgs& a, int b, int& before, int& total) {
-  const int lane = threadIdx.x & 63;
-  before = total = 0;
-  for (int b0 = 0; b0 < a.c.B; b0 += 64) {
-    const int n = units_of(a, b0 + lane);
-    const int x = wave_prefix(n, lane);
-    if (b >= b0 && b < b0 + 64) before = total + __builtin_amdgcn_readfirstlane(__shfl(x - n, b - b0));
-    total += __builtin_amdgcn_readfirstlane(__shfl(x, 63));
-  }
+// Units of all sequences (every lane of the wave calls).
+__device__ __forceinline__ int total_units(const PagedAttnArgs& a) {
+  int n = 0;
+#pragma unroll 4
+  for (int b0 = 0; b0 < a.c.B; b0 += 64) n += units_of(a, b0 + (threadIdx.x & 63));
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) n += __shfl_xor(n, o);
+  return __builtin_amdgcn_readfirstlane(n);
 }
 
 // The sequence that holds unit u < total, and its first unit.
@@ -431,8 +429,7 @@ __global__ __launch_bounds__(64 * WAVES) void paged_attn_kernel(const PagedAttnA
     start = u = 0;
     end = 1;
   } else {
-    int none, total;
-    units_before(a, 0, none, total);
+    const int total = total_units(a);
     per = units_per_part(total, a.parts, a.least);
     once = total > a.keep_units;
     if (int64_t(part) * per >= total) return;
@@ -442,14 +439,18 @@ __global__ __launch_bounds__(64 * WAVES) void paged_attn_kernel(const PagedAttnA
   }
 
   Wave<E, D, RT> w;
-  // (b < B, v0 >= 0 and the join's last part hold by themselves, unless lens change under a running call: then the results
-  // mean nothing, but no access leaves the tensors)
+  // (b < B and v0 >= 0 hold by themselves, and so do the bounds in pieces_of, unless lens change under a running call: then the
+  // results mean nothing, but no access leaves the tensors)
   while (u < end && b < a.c.B) {
     const Visible vis = visible(seq_len(a.c, b), a.W, a.S);
     const int units = paged_units(vis.count);
     if (a.parts == 0) end = units;
     const int stop = imin(end, start + units);
     const bool whole = u == start && stop == start + units;
+    if (a.parts && stream == 0 && tid == 0) {  // for the second launch
+      if (u == start) a.starts[b] = start;
+      if (u == 0) a.starts[a.c.B] = per;
+    }
     const int v0 = imax(0, (u - start) * kPagedUnit), v1 = imin(vis.count, (stop - start) * kPagedUnit);
 #pragma unroll
     for (int x = 0; x < RT; ++x) {
@@ -589,11 +590,10 @@ struct Pieces {
 __device__ __forceinline__ Pieces pieces_of(const PagedAttnArgs& a, int b) {
   Pieces p{0, 0, 0, 0};
   if (a.parts == 0) return p;
-  int total;
-  units_before(a, b, p.start, total);
-  p.per = units_per_part(total, a.parts, a.least);
-  p.first = p.start / p.per;
-  p.last = imin(a.parts - 1, (p.start + units_of(a, b) - 1) / p.per);
+  p.start = a.starts[b];
+  p.per = imax(1, a.starts[a.c.B]);
+  p.first = imin(imax(p.start / p.per, 0), a.parts - 1);
+  p.last = imin((p.start + units_of(a, b) - 1) / p.per, a.parts - 1);
   return p;
 }
 

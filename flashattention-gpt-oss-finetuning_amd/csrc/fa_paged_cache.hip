@@ -61,19 +61,24 @@ __device__ __forceinline__ u32x2 encode8(u32x4 x, float inv) {
 }
 
 // The sequence of packed row `row` (cu: [B + 1] offsets) and how many of the sequence's rows lie behind it, or -1 where the
-// row is no sequence's.  Every lane of the wave calls.
+// row is no sequence's: the first b with cu[b + 1] > row, by ballots that narrow the range to a 64th.  Every lane of the
+// wave calls.
 __device__ __forceinline__ int row_seq(const int* cu, int B, int row, int& behind) {
   const int lane = threadIdx.x & 63;
-  for (int b0 = 0; b0 < B; b0 += 64) {
-    const int end = b0 + lane < B ? cu[b0 + lane + 1] : -1;
+  int lo = 0, n = B;  // it is among sequences [lo, lo + n)
+  while (true) {
+    const int step = (n + 63) / 64, at = imin(n, (lane + 1) * step);
+    const int end = cu[lo + at];  // the end of the last sequence of the lane's share
     const unsigned long long m = __ballot(end > row);
-    if (m) {
-      const int l = __builtin_amdgcn_readfirstlane(__ffsll(m) - 1);
+    if (!m) return -1;
+    const int l = __builtin_amdgcn_readfirstlane(__ffsll(m) - 1);
+    lo += l * step;
+    n = imin(step, n - l * step);
+    if (n == 1) {
       behind = __builtin_amdgcn_readfirstlane(__shfl(end, l)) - row;
-      return cu[b0 + l] <= row ? b0 + l : -1;
+      return cu[lo] <= row ? lo : -1;
     }
   }
-  return -1;
 }
 
 // PP: 16-byte pieces of a head's source row.  T: void for pages of the source's type, else the source's type for e4m3 pages.

@@ -525,6 +525,13 @@ void changed(const at::Tensor& t) {
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
+// Entries of `t` that share memory cannot be written.
+void distinct(const at::Tensor& t, const char* name) {
+  for (int64_t d = 0; d < t.dim(); ++d)
+    if (t.stride(d) == 0 && t.size(d) > 1)
+      throw std::invalid_argument(std::string(name) + " is written in place: its entries must not share memory (an expanded tensor)");
+}
+
 // The cache's parameter block.  block_table and lens are copied where their entries are not next to each other; the copies
 // are kept in `keep` for the call.
 fa_paged_cache paged_cache(const at::Tensor& k_pages, const at::Tensor& v_pages, const at::Tensor& table,
@@ -604,6 +611,8 @@ void paged_append(const at::Tensor& k_in, const at::Tensor& v_in, const at::Tens
   refuse_transformed({&k_in, &v_in, &k_pages, &v_pages}, "paged_append");
   std::vector<at::Tensor> keep;
   const fa_paged_cache c = paged_cache(k_pages, v_pages, table, lens, k_descale, v_descale, keep);
+  distinct(k_pages, "k_pages");
+  distinct(v_pages, "v_pages");
   const c10::DeviceGuard guard(k_pages.device());
   const at::Tensor k = paged_input(k_in, k_pages, "k"), v = paged_input(v_in, k_pages, "v");
   if (k.size(1) != k_pages.size(1) || v.sizes() != k.sizes() || v.scalar_type() != k.scalar_type())
@@ -650,6 +659,7 @@ at::Tensor paged_attention(const at::Tensor& q_in, const at::Tensor& k_pages, co
         (sums->stride(2) != 1 && sums->size(2) != 1))
       throw std::invalid_argument("weight_sums must be float32 [B, Hkv, tokens], next to each other in the last dimension, got " +
                                   shape_of(*sums));
+    distinct(*sums, "weight_sums");
     p.weight_sums = sums->data_ptr<float>();
     p.sums_stride[0] = sums->stride(0);
     p.sums_stride[1] = sums->stride(1);
@@ -676,6 +686,8 @@ std::vector<at::Tensor> paged_evict(const at::Tensor& k_pages, const at::Tensor&
   std::vector<at::Tensor> keep;
   fa_paged_evict_params p{};
   p.cache = paged_cache(k_pages, v_pages, table, lens, 1.0, 1.0, keep);
+  distinct(k_pages, "k_pages");
+  distinct(v_pages, "v_pages");
   const c10::DeviceGuard guard(k_pages.device());
   on_device(sums, k_pages, "weight_sums", "k_pages");
   on_device(new_table_in, k_pages, "new_table", "k_pages");

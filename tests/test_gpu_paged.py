@@ -568,6 +568,12 @@ def test_refusals(fa, gpu, monkeypatch, binding):
                     (dict(weight_sums=sums.cpu()), RuntimeError), (dict(weight_sums=torch.zeros(2, 48, 2, device=gpu).transpose(1, 2)), ValueError)):
         with pytest.raises(err):
             att(**kw)
+    wide = kp[:1].expand(6, 2, 16, 64)
+    for f, kw in ((app, dict(k_pages=wide)), (app, dict(v_pages=wide)), (evi, dict(k_pages=wide)), (evi, dict(v_pages=wide)),
+                  (att, dict(weight_sums=sums[:1].expand(2, 2, 48)))):
+        with pytest.raises(ValueError, match="share memory"):
+            f(**kw)
+    att(k_pages=wide, v_pages=wide)  # (reading them is well defined)
     q8 = torch.zeros(6, 2, 16, 64, device=gpu).to(torch.float8_e4m3fn)
     with pytest.raises(ValueError):
         att(q=q.float(), k_pages=q8, v_pages=q8)
@@ -608,3 +614,58 @@ def test_ctypes_path(fa, gpu, monkeypatch):
     monkeypatch.setattr(load_mod("_ops"), "_BINDING", None)
     for y, z in zip(a, run()):
         same(y, z)
+
+
+def test_inputs_in_other_layouts(fa, gpu):
+    """q, k, v, the table and lens as views: slices of a fused projection, unaligned, strided."""
+    c = make(81, "bf16", "bf16", 64, 8, 2, 16, "hnd", (700, 33, 5), nan=False)
+    kp, vp, t, lens = (c[n].to(gpu) for n in ("kp", "vp", "table", "lens"))
+    q = c["q"].to(gpu)
+    want = fa.paged_attention(q, kp, vp, t, lens)
+    k, v = (torch.randn(3, 2, 64, generator=c["g"]).to(torch.bfloat16).to(gpu) for _ in range(2))
+    fused = torch.cat((q, k, v), 1)  # [B, Hq + 2 Hkv, D]
+    odd = torch.zeros(3 * 8 * 64 + 1, dtype=torch.bfloat16, device=gpu)[1:].view(3, 8, 64).copy_(q)
+    by_dim = q.transpose(1, 2).contiguous().transpose(1, 2)
+    one = torch.zeros(3, 8, 64, 2, dtype=torch.bfloat16, device=gpu)[..., 0].copy_(q)
+    wide = torch.zeros(3, t.shape[1], 2, dtype=torch.int32, device=gpu)[..., 1].copy_(t)
+    turned = t.t().contiguous().t()
+    far = torch.zeros(3, 2, dtype=torch.int32, device=gpu)[:, 1].copy_(lens)
+    for x in (fused[:, :8], odd, by_dim, one, q.unsqueeze(2).expand(3, 8, 5, 64)[:, :, 3]):
+        for tt in (t, wide, turned):
+            same(fa.paged_attention(x, kp, vp, tt, far), want)
+    a, b = (kp.clone(), vp.clone()), (kp.clone(), vp.clone())
+    fa.paged_append(k, v, *a, t, lens)
+    strange = torch.zeros(3, 2, 64, 3, dtype=torch.bfloat16, device=gpu)[..., 2].copy_(k)
+    fa.paged_append(strange, fused[:, 10:], *b, wide, far)
+    same(a[0], b[0])
+    same(a[1], b[1])
+
+
+def test_shared_prefix(fa, gpu):
+    """Two sequences share the pages of a prefix: attention reads them, eviction leaves them whole."""
+    c = make(82, "bf16", "bf16", 64, 4, 2, 16, "hnd", (100, 90), nan=False)
+    c["table"][1, :4] = c["table"][0, :4]
+    P = c["kp"].shape[0]
+    kp, vp = (torch.cat((x, x[:6])) for x in (c["kp"], c["vp"]))
+    sums = torch.rand(2, 2, 112, generator=c["g"])
+    new_table = torch.arange(P, P + 6, dtype=torch.int32).view(2, 3)
+    t, lens, gk, gv, gs = c["table"].to(gpu), c["lens"].to(gpu), kp.to(gpu), vp.to(gpu), sums.to(gpu)
+    ref, mag, ref_sums = oracle.attention(c["q"], kp, vp, c["table"], c["lens"], sums=sums)
+    o = fa.paged_attention(c["q"].to(gpu), gk, gv, t, lens, weight_sums=gs)
+    check_attention(o, dict(c, kp=kp, vp=vp), ref, mag, "bf16", 64, 100, 0.125)
+    assert torch.allclose(gs.cpu().double(), ref_sums, rtol=1e-5, atol=1e-6)
+    want = oracle.evict(kp, vp, c["table"], c["lens"], gs.cpu(), 48, new_table, 4, 8)
+    left, new = fa.paged_evict(gk, gv, t, lens, gs, 48, new_table.to(gpu), 4, 8)
+    same(gk, want[0])
+    same(gv, want[1])
+    same(new, want[3])
+
+
+def test_traced_calls_are_refused(fa, gpu):
+    kp = torch.zeros(4, 2, 16, 64, dtype=torch.bfloat16, device=gpu)
+    t, lens = torch.zeros(1, 2, dtype=torch.int32, device=gpu), torch.ones(1, dtype=torch.int32, device=gpu)
+    q = torch.zeros(1, 4, 64, dtype=torch.bfloat16, device=gpu)
+    with pytest.raises(RuntimeError, match="traced"):
+        torch.jit.trace(lambda x: fa.paged_attention(x, kp, kp, t, lens), (q,), check_trace=False)
+    with pytest.raises(RuntimeError, match="traced"):
+        torch.func.vmap(lambda x: fa.paged_attention(x, kp, kp, t, lens))(q.unsqueeze(0))
