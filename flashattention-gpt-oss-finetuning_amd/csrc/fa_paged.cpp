@@ -65,17 +65,25 @@ fa::PagedCache cache_args(const fa_paged_cache& c) {
 
 int status(hipError_t e) { return e == hipSuccess ? FA_OK : FA_ERR_LAUNCH; }
 
-// Sequences of at most so many visible keys are taken whole, a workgroup each, in one launch: kWholeKeys, or kWholeMany
-// where there are at least kManyWgs (KV head, row tile, sequence) triples.
+// Which launch serves a call.  Times in us of a call with D = 64, bf16, Hq = 64, Hkv = 8, whole / split:
+//   1 sequence of 1001 tokens 7.9 / 9.1, of 1500 9.4 / 9.1, of 2048 11.3 / 9.2; 4 of 2048 11.4 / 10.0;
+//   16 (128 workgroups) of 1500 11.7 / 16.3, of 2048 14.4 / 19.0; 64 (512 workgroups) of 2048 43.9 / 48.1, of 4096 97 / 85.
+// So sequences of at most kWholeKeys visible keys are taken whole, a workgroup each, in one launch; of at most kWholeMany
+// where there are kManyWgs (KV head, share of its heads, sequence) triples.  Ragged batches are no reason to split here: the bound is what
+// the longest can be.
 constexpr int kWholeKeys = 1024, kWholeMany = 2048, kManyWgs = 128;
-// Workgroups of a split call's launch for each compute unit (more for rows of 32 bytes, whose tiles are as much work and a
-// quarter of the bytes of D = 64), and the fewest units worth a workgroup of their own.
-constexpr int kPartsPerCu = 2, kPartsNarrow = 3, kLeastUnits = 1;
-
-// Whole sequences of at most kSingleUnits units are taken by one wave each where there are kSingleWgs of them.
+// Whole sequences are taken by 8 waves while there are at most as many workgroups as compute units (1 sequence of 1001
+// tokens: 9.2 us with 4 waves, 7.9 with 8; but 64 of 256: 7.4 and 9.5), and by a wave each where there are kSingleWgs of at
+// most kSingleUnits units (256 sliding-layer sequences 17.7 us with 4 waves, 14.2 with one; 1024 of them 78 and 59).
 constexpr int kSingleWgs = 1024, kSingleUnits = 2;
-
-// K and V bytes up to which a call's loads leave them in the 256 MB last-level cache, for the next step to find.
+// Split calls: workgroups for each compute unit.  With 1 / 2 / 3 of them 32 ragged sequences (261 MB) take 54 / 49 / 55 us, e4m3
+// D = 128 (123 MB) 30 / 27 / 33, four of up to 128K tokens (876 MB) 160 / 157 / 148.  Rows of 32 bytes make a tile as much work for a
+// quarter of the bytes: 137 us with 2, 113 with 3 (537 MB).  A unit more a workgroup costs a short call more than its piece
+// does (1 sequence of 2048 tokens: 10.3 us with at least two units each, 9.8 with one).
+constexpr int kPartsPerCu = 2, kPartsNarrow = 3, kLeastUnits = 1;
+// Loads of a call that reads more than this are marked as read once, so that they do not run through the 256 MB last-level
+// cache: 537 MB take 84 us so and 103 otherwise, 261 MB 49 and 54.  Below, the next step finds the keys there: three caches of 71 MB
+// in turn take 17.4 us each, 19.3 with marked loads.
 constexpr int64_t kKeepBytes = int64_t(96) << 20;
 
 struct Plan {
@@ -115,7 +123,8 @@ int plan(const fa_paged_attention_params* p, Plan* r) {
   r->parts = 0;
   if (most > (streams * c.batch >= kManyWgs ? kWholeMany : kWholeKeys)) {
     const int64_t want = std::max<int64_t>(1, int64_t(c.head_dim * elem_bytes(c.dtype) <= 32 ? kPartsNarrow : kPartsPerCu) * fa::device_cus() / streams);
-    // (whole rounds of the 8 XCDs: the tiles of a group's heads then read the same keys through one L2)
+    // (whole rounds of the 8 XCDs: the workgroups of a part, which read the same or neighbouring entries, then share an L2; pages
+    // with the slots before the heads, 876 MB: 166 us with a KV head an XCD, 158 so)
     r->parts = int((std::min(want, (units + kLeastUnits - 1) / kLeastUnits) + 7) / 8 * 8);
     if (!fa::grid_fits(streams * r->parts)) return FA_ERR_OVERFLOW;
   }

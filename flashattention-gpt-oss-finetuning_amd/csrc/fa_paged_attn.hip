@@ -5,8 +5,7 @@
 // 4 G operations a cache element, so the cache's bytes bound it: the kernel is built to keep them coming.
 //
 // paged_attn_kernel.  A workgroup of 4 or 8 waves takes a run of keys for 16 query heads (a group, padded); its waves
-// take tiles of 32 keys in turn and meet only at the run's end.  A tile goes from memory to registers to the
-// matrix instructions, without LDS and without a lane seeing another's values:
+// take tiles of 32 keys in turn and meet only at the run's end.  In between no lane needs another's values:
 //   * S^T = K Q^T as v_mfma_f32_16x16x32 with the keys as rows.  Lane l (r = l % 16, j = l / 16) supplies key rows r of two
 //     16-key halves and gets, for head r, rows 4j..4j+3 of both.  Half T's row 4j + i is the tile's key 8j + 4T + i, so the
 //     lane's eight scores are those of keys 8j..8j+7.
@@ -14,8 +13,10 @@
 //     operand is eight V entries of keys 8j..8j+7, of which the lane loads D / 16 neighbouring dims each and pairs
 //     two keys' halves (one v_perm per register).  Its C rows are the lane's own head again, so
 //     maximum, sum and rescaling need no exchange.
-// The running maximum is raised only where a score exceeds it by more than 2^8 (weights stay within float32 and
-// 16 bits), which after the first tiles hardly ever happens; only then do lanes exchange maxima.
+// The running maximum is raised only where a key's weight against it would exceed 2^8 (which 16 bits and float32 hold as
+// well as 1), after the first tiles hardly ever; only then do lanes exchange maxima.
+// K is loaded with neighbouring lanes on neighbouring 16-byte pieces and turned into fragments in the wave's own LDS: loaded
+// as fragments (16 rows an instruction) 876 MB took 190 us, so 166.
 // P goes into the 16-bit product as the sum of two 16-bit parts (P rounded, and what that left), so o carries its own
 // rounding only; the second product costs matrix time that the loads leave idle.  float32 uses v_mfma_f32_16x16x4.
 //
@@ -28,6 +29,12 @@
 // (fa_paged_plan.h): each workgroup finds its run by a prefix sum over lens, on the device, so the grid depends on
 // sizes the host knows.  Pieces that are no whole sequence leave (maximum, sum, o) in the workspace, and
 // paged_finish_kernel joins them.
+//
+// Measured (D = 64, bf16, 8 heads a group; rocprofv3): 32 ragged sequences, 261 MB of K and V, 49 to 51 us, 5.2 TB/s; four of up to 128K
+// tokens, 876 MB, 142 us with the heads before the slots in a page, 6.2 TB/s, and 157 with the slots first.  The
+// counters show 261 and 877 MB read: every entry once.  A plain kernel that only reads reaches 6.2 TB/s, 7.1 with loads marked as read
+// once.  Without the products and the softmax (loads only) the kernel took the same time to 3%.
+// What is left of a small call is latency: lens, table, K, four tiles, the waves' sums: one sliding-layer step 5.3 us.
 #include <hip/hip_runtime.h>
 
 #include "../../include/fa_gfx950.h"
@@ -135,7 +142,8 @@ struct Tile {
   static constexpr int NK = STAGED ? PR / 2 : 2 * NF;        // pieces of the tile that a lane loads
   static constexpr int VB = ROW / 16;                        // bytes of a V entry that a lane holds
   static constexpr int VD = VB >= 4 ? VB / 4 : 1;
-  static constexpr int AHEAD = ROW <= 64 ? 4 : 2;  // tiles in flight, of 4 to 64 registers each way
+  // tiles in flight (D = 32, 268 MB: 50.8 us with 2, 48.8 with 4; D = 64 in 16 bits no gain, D = 128 in 8 bits 24.6 and 31.4)
+  static constexpr int AHEAD = ROW <= 64 ? 4 : 2;
   u32x4 k[NK];
   uint32_t v[8][VD];
   uint32_t live;  // bit i: key i of the tile is on a page (the same in every lane)
