@@ -669,3 +669,17 @@ def test_traced_calls_are_refused(fa, gpu):
         torch.jit.trace(lambda x: fa.paged_attention(x, kp, kp, t, lens), (q,), check_trace=False)
     with pytest.raises(RuntimeError, match="traced"):
         torch.func.vmap(lambda x: fa.paged_attention(x, kp, kp, t, lens))(q.unsqueeze(0))
+
+
+def test_inference_mode(fa, gpu):
+    """Inference tensors have no version counters to raise."""
+    c = make(91, "bf16", "bf16", 64, 4, 2, 16, "hnd", (40, 9), nan=False)
+    with torch.inference_mode():
+        kp, vp, t, lens = (c[n].to(gpu) for n in ("kp", "vp", "table", "lens"))
+        x = torch.randn(2, 2, 64, generator=c["g"]).to(torch.bfloat16).to(gpu)
+        sums = torch.zeros(2, 2, t.shape[1] * 16, device=gpu)
+        fa.paged_append(x, x, kp, vp, t, lens)
+        fa.paged_attention(c["q"].to(gpu), kp, vp, t, lens, weight_sums=sums)
+        nt = torch.arange(c["used"], c["used"] + 2, dtype=torch.int32, device=gpu).view(2, 1)
+        left, new = fa.paged_evict(kp, vp, t, lens, sums, 16, nt)
+        assert left.tolist() == [16, 9] and float(sums.sum()) > 0
