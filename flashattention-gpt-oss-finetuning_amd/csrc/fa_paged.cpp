@@ -88,8 +88,8 @@ constexpr int64_t kKeepBytes = int64_t(96) << 20;
 
 struct Plan {
   int max_units, row_tiles, rt, parts;
-  size_t starts, part_o, part_ml, lse, logits;  // bytes
-  size_t bytes() const { return std::max<size_t>(256, starts + part_o + part_ml + lse + logits); }
+  size_t starts, part_o, part_ml, norm, logits;  // bytes
+  size_t bytes() const { return std::max<size_t>(256, starts + part_o + part_ml + norm + logits); }
 };
 
 int plan(const fa_paged_attention_params* p, Plan* r) {
@@ -119,7 +119,7 @@ int plan(const fa_paged_attention_params* p, Plan* r) {
   r->row_tiles = (G + 15) / 16;
   r->rt = r->row_tiles > 1 && fa::paged_pairs(c.head_dim, elem_bytes(c.dtype)) ? 2 : 1;
   const int64_t streams = int64_t(c.heads_kv) * ((r->row_tiles + r->rt - 1) / r->rt), units = int64_t(c.batch) * r->max_units;
-  if (units >= (int64_t(1) << 31) || !fa::grid_fits(std::max(streams, int64_t(p->heads_q)) * c.batch)) return FA_ERR_OVERFLOW;
+  if (units >= (int64_t(1) << 30) || !fa::grid_fits(std::max(streams, int64_t(p->heads_q)) * c.batch)) return FA_ERR_OVERFLOW;
   r->parts = 0;
   if (most > (streams * c.batch >= kManyWgs ? kWholeMany : kWholeKeys)) {
     const int64_t want = std::max<int64_t>(1, int64_t(c.head_dim * elem_bytes(c.dtype) <= 32 ? kPartsNarrow : kPartsPerCu) * fa::device_cus() / streams);
@@ -132,9 +132,9 @@ int plan(const fa_paged_attention_params* p, Plan* r) {
   r->starts = r->parts ? align256((size_t(c.batch) + 1) * sizeof(int32_t)) : 0;
   r->part_o = align256(slots * 16 * c.head_dim * sizeof(float));
   r->part_ml = align256(slots * 32 * sizeof(float));
-  r->lse = r->logits = 0;
+  r->norm = r->logits = 0;
   if (p->weight_sums) {
-    r->lse = align256(size_t(c.batch) * p->heads_q * sizeof(float));
+    r->norm = align256(size_t(c.batch) * p->heads_q * 2 * sizeof(float));
     r->logits = align256(size_t(units) * p->heads_q * fa::kPagedUnit * sizeof(float));
     // (the second launch: a workgroup a query head, and one for each 1024 keys of a (sequence, KV head))
     if (!fa::grid_fits((p->heads_q + int64_t(r->max_units + 7) / 8 * c.heads_kv) * c.batch)) return FA_ERR_OVERFLOW;
@@ -241,8 +241,8 @@ int fa_paged_attention(const fa_paged_attention_params* p, void* workspace, size
   a.starts = reinterpret_cast<int*>(ws);
   a.part_o = reinterpret_cast<float*>(ws += r.starts);
   a.part_ml = reinterpret_cast<float*>(ws += r.part_o);
-  a.lse = reinterpret_cast<float*>(ws += r.part_ml);
-  a.logits = reinterpret_cast<float*>(ws += r.lse);
+  a.norm = reinterpret_cast<float*>(ws += r.part_ml);
+  a.logits = reinterpret_cast<float*>(ws += r.norm);
   return status(fa::launch_paged_attention(a, p->dtype, c.dtype, c.head_dim, static_cast<hipStream_t>(stream)));
 }
 

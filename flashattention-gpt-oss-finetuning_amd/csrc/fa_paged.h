@@ -56,7 +56,7 @@ struct PagedAttnArgs {
   int* starts;            // split calls: [B] the sequences' first units, and the units of a part
   float* part_o;          // [Hkv row_tiles][parts][2][16][D]
   float* part_ml;         // [Hkv row_tiles][parts][2][2][16]: maximum (log2 domain), sum
-  float* lse;             // with sums: [B][Hq] (log2 domain), of the sequences that one workgroup took whole
+  float* norm;            // with sums: [B][Hq] maximum (log2 domain) and 1 / sum, of the sequences that one workgroup took whole
   float* logits;          // with sums: [Hkv][B][max_units][G][kPagedUnit] (log2 domain)
 };
 

@@ -570,7 +570,8 @@ __global__ __launch_bounds__(64 * WAVES) void paged_attn_kernel(const PagedAttnA
 #pragma unroll
           for (int c = 0; c < NC; ++c) o[c] = sum == 0.f ? 0.f : o[c] * inv;
           store_out<E, NC>(a.o + int64_t(b) * a.so[0] + int64_t(hq) * a.so[1] + od * E::EB, o);
-          if (a.sums && (y & 15) == 0) a.lse[int64_t(b) * a.Hq + hq] = (m == kNegInf ? 0.f : m) + fast_log2(ls);
+          if (a.sums && (y & 15) == 0)
+            *reinterpret_cast<f32x2*>(a.norm + 2 * (int64_t(b) * a.Hq + hq)) = f32x2{m == kNegInf ? 0.f : m, ls == 0.f ? 0.f : 1.f / ls};
         } else {
           const int64_t slot = (int64_t(hkv) * a.row_tiles + h / 16) * a.parts * 2 + part_slot(part, per, start);
           float* po = a.part_o + (slot * 16 + oh) * D + od;
@@ -648,10 +649,10 @@ __device__ __forceinline__ void join_head(const PagedAttnArgs& a, int b, int hq,
   }
 }
 
-// sums[b, hkv, key] += sum over the group's heads of 2^(logit - lse): a thread takes keys, so there is no order to choose and
-// no atomic.
+// sums[b, hkv, key] += sum over the group's heads of 2^(logit - maximum) / sum: a thread takes keys, so there is no order to
+// choose and no atomic.
 constexpr int kSumKeys = 1024;
-constexpr int kSumHeads = 16;  // heads at a time: 16 threads work out a head's lse
+constexpr int kSumHeads = 16;  // heads at a time: 16 threads work out a head's maximum and the reciprocal of its sum
 __device__ __forceinline__ void add_weights(const PagedAttnArgs& a, int b, int hkv, int chunk, float* smem) {
   const Visible vis = visible(seq_len(a.c, b), a.W, a.S);
   if (chunk * kSumKeys >= vis.count) return;
@@ -665,7 +666,7 @@ __device__ __forceinline__ void add_weights(const PagedAttnArgs& a, int b, int h
   const Pieces ps = pieces_of(a, b);
   for (int g0 = 0; g0 < a.G; g0 += kSumHeads) {
     const int ng = imin(kSumHeads, a.G - g0);
-    constexpr int HELD = 8;  // scores asked for before the lse are known
+    constexpr int HELD = 8;  // scores asked for before those are known
     f32x4 s[HELD];
 #pragma unroll
     for (int i = 0; i < HELD; ++i) s[i] = *reinterpret_cast<const f32x4*>(x + (g0 + imin(i, ng - 1)) * kPagedUnit);
@@ -673,9 +674,11 @@ __device__ __forceinline__ void add_weights(const PagedAttnArgs& a, int b, int h
     const int g = g0 + int(threadIdx.x) / 16, sub = threadIdx.x & 15;
     if (g < a.G) {
       const int hq = hkv * a.G + g;
-      float lse;
+      float top, inv;
       if (ps.first >= ps.last) {
-        lse = a.lse[int64_t(b) * a.Hq + hq];
+        const f32x2 v = *reinterpret_cast<const f32x2*>(a.norm + 2 * (int64_t(b) * a.Hq + hq));
+        top = v[0];
+        inv = v[1];
       } else {
         const float* ml = a.part_ml + int64_t(hkv * a.row_tiles + g / 16) * a.parts * 2 * 32 + g % 16;
         float m = a.sinks ? a.sinks[hq] * kLog2e : kNegInf;
@@ -691,15 +694,19 @@ __device__ __forceinline__ void add_weights(const PagedAttnArgs& a, int b, int h
         }
 #pragma unroll
         for (int y = 8; y >= 1; y >>= 1) l += __shfl_xor(l, y);
-        lse = ref + fast_log2(l);
+        top = ref;
+        inv = l == 0.f ? 0.f : 1.f / l;
       }
-      if (sub == 0) smem[g - g0] = lse;
+      if (sub == 0) {
+        smem[g - g0] = top;
+        smem[kSumHeads + g - g0] = inv;
+      }
     }
     __syncthreads();
     auto add = [&](f32x4 q, int i) {
-      const float lse = smem[i];
+      const float top = smem[i], inv = smem[kSumHeads + i];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) w[c] += q[c] == kNegInf ? 0.f : fast_exp2(q[c] - lse);
+      for (int c = 0; c < 4; ++c) w[c] += q[c] == kNegInf ? 0.f : fast_exp2(q[c] - top) * inv;
     };
 #pragma unroll
     for (int i = 0; i < HELD; ++i)
