@@ -65,13 +65,20 @@ fa::PagedCache cache_args(const fa_paged_cache& c) {
 
 int status(hipError_t e) { return e == hipSuccess ? FA_OK : FA_ERR_LAUNCH; }
 
-// Which launch serves a call.  Times in us of a call with D = 64, bf16, Hq = 64, Hkv = 8, whole / split:
-//   1 sequence of 1001 tokens 7.9 / 9.1, of 1500 9.4 / 9.1, of 2048 11.3 / 9.2; 4 of 2048 11.4 / 10.0;
-//   16 (128 workgroups) of 1500 11.7 / 16.3, of 2048 14.4 / 19.0; 64 (512 workgroups) of 2048 43.9 / 48.1, of 4096 97 / 85.
-// So sequences of at most kWholeKeys visible keys are taken whole, a workgroup each, in one launch; of at most kWholeMany
-// where there are kManyWgs (KV head, share of its heads, sequence) triples.  Ragged batches are no reason to split here: the bound is what
-// the longest can be.
-constexpr int kWholeKeys = 1024, kWholeMany = 2048, kManyWgs = 128;
+// Which launch serves a call.  Sequences that see at most whole_keys() keys are taken whole, a workgroup each, in one launch; twice
+// as many where there are kManyWgs (KV head, share of its heads, sequence) triples.  Ragged batches are no reason to split here: the
+// bound is what the longest can be.  Times in us, whole / split, with 8 KV heads and D = 64 (4 and D = 128):
+//   bf16: 1 sequence of 1001 tokens 7.9 / 9.1, of 1500 9.4 / 9.1, of 2048 11.3 / 9.2; 4 of 2048 11.4 / 10.0;
+//     16 (128 workgroups) of 1500 11.7 / 16.3, of 2048 14.4 / 19.0; 64 (512 workgroups) of 2048 43.9 / 48.1, of 4096 97 / 85
+//   bf16 D = 128: 1 of 600 9.4 / 9.3, of 1000 12.6 / 9.5; 16 (64 workgroups) of 1000 13.4 / 16.0, of 2000 22.6 / 23.2
+//   e4m3 D = 128: 1 of 600 8.0 / 9.2, of 1000 10.4 / 9.3; 16 (64 workgroups) of 1000 10.8 / 11.2, of 1500 14.0 / 12.8
+//   float32: 1 of 600 12.6 / 10.0 (the lines cross at about 380); 16 (128 workgroups) of 600 14.0 / 17.6, of 1000 19.6 / 20.0;
+//     D = 128: 1 of 600 21.6 / 12.4
+//   64 heads over one: 1 of 600 8.7 / 10.8, of 1000 11.0 / 10.9; 16 of 1000 11.4 / 12.2, of 1500 14.1 / 13.7
+int whole_keys(int D, int cache_bytes) {
+  return cache_bytes == 4 ? 256 : D * cache_bytes > 128 ? 512 : D > 64 ? 768 : 1024;
+}
+constexpr int kManyWgs = 128;
 // Whole sequences are taken by 8 waves while there are at most as many workgroups as compute units (1 sequence of 1001
 // tokens: 9.2 us with 4 waves, 7.9 with 8; but 64 of 256: 7.4 and 9.5), and by a wave each where there are kSingleWgs of at
 // most kSingleUnits units (256 sliding-layer sequences 17.7 us with 4 waves, 14.2 with one; 1024 of them 78 and 59).
@@ -121,7 +128,7 @@ int plan(const fa_paged_attention_params* p, Plan* r) {
   const int64_t streams = int64_t(c.heads_kv) * ((r->row_tiles + r->rt - 1) / r->rt), units = int64_t(c.batch) * r->max_units;
   if (units >= (int64_t(1) << 30) || !fa::grid_fits(std::max(streams, int64_t(p->heads_q)) * c.batch)) return FA_ERR_OVERFLOW;
   r->parts = 0;
-  if (most > (streams * c.batch >= kManyWgs ? kWholeMany : kWholeKeys)) {
+  if (most > whole_keys(c.head_dim, elem_bytes(c.dtype)) * (streams * c.batch >= kManyWgs ? 2 : 1)) {
     const int64_t want = std::max<int64_t>(1, int64_t(c.head_dim * elem_bytes(c.dtype) <= 32 ? kPartsNarrow : kPartsPerCu) * fa::device_cus() / streams);
     // (whole rounds of the 8 XCDs: the workgroups of a part, which read the same or neighbouring entries, then share an L2; pages
     // with the slots before the heads, 876 MB: 166 us with a KV head an XCD, 158 so)
@@ -234,8 +241,10 @@ int fa_paged_attention(const fa_paged_attention_params* p, void* workspace, size
   a.max_units = r.max_units;
   a.parts = r.parts;
   a.least = kLeastUnits;
-  const int64_t wgs = int64_t(c.heads_kv) * r.row_tiles * c.batch;
-  a.waves = r.parts ? 4 : wgs <= fa::device_cus() ? 8 : wgs >= kSingleWgs && r.max_units <= kSingleUnits ? 1 : 4;
+  const int64_t wgs = int64_t(c.heads_kv) * ((r.row_tiles + r.rt - 1) / r.rt) * c.batch;
+  if (r.parts) a.waves = 4;
+  else if (wgs <= fa::device_cus() && fa::paged_eight(c.head_dim, elem_bytes(c.dtype), r.rt)) a.waves = 8;
+  else a.waves = r.rt == 1 && wgs >= kSingleWgs && r.max_units <= kSingleUnits ? 1 : 4;
   a.keep_units = int(std::min<int64_t>(kKeepBytes / (int64_t(fa::kPagedUnit) * 2 * c.head_dim * elem_bytes(c.dtype) * c.heads_kv), INT32_MAX));
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   a.starts = reinterpret_cast<int*>(ws);

@@ -33,6 +33,11 @@ struct AppendArgs {
 
 // Two tiles of heads and their sums fit a wave's registers: more than 16 heads a group then share what is read.
 constexpr bool paged_pairs(int D, int cache_bytes) { return cache_bytes <= 2 && D * cache_bytes <= 128; }
+// A wave of a workgroup of 8 has 256 registers: no room for two tiles of heads with D = 128, nor for 16-bit and
+// float32 rows of that.
+constexpr bool paged_eight(int D, int cache_bytes, int rt) {
+  return cache_bytes == 4 ? D <= 64 : D * cache_bytes <= 128 && (D <= 64 || rt == 1);
+}
 
 struct PagedAttnArgs {
   PagedCache c;
@@ -49,7 +54,7 @@ struct PagedAttnArgs {
   int max_units;          // units of a sequence of max_len tokens
   // split calls: the runs a (KV head, row tile) is cut into, 0 where every workgroup takes a whole sequence
   int parts, least;
-  int waves;              // of a workgroup: 1, 4 or 8
+  int waves;              // of a workgroup: 1 (only with rt = 1), 4 or 8 (paged_eight)
   int rt;                 // tiles of heads that a workgroup takes: 1, or 2 (paged_pairs)
   int keep_units;         // calls that read more units a KV head than this mark their loads as read once
   // workspace

@@ -737,13 +737,16 @@ hipError_t run(const PagedAttnArgs& a, hipStream_t s) {
   const unsigned B = unsigned(a.c.B), parts = a.parts ? unsigned(a.parts) : B;
   const unsigned streams = unsigned(a.c.Hkv) * unsigned((a.row_tiles + a.rt - 1) / a.rt);
   const auto launch = [&](auto kernel, int waves) { hipLaunchKernelGGL(kernel, dim3(streams * parts), dim3(64 * waves), 0, s, a); };
-  constexpr bool EIGHT = sizeof(Shared<E, D, 8>) <= 65536;  // (the waves' tables and tiles in LDS)
-  const int waves = a.rt == 2 || (a.waves == 8 && !EIGHT) ? 4 : a.waves;
   if (a.rt == 2) {
-    if constexpr (paged_pairs(D, E::CB)) launch(paged_attn_kernel<E, D, 4, 2>, 4);
-  } else if (waves == 8) {
-    if constexpr (EIGHT) launch(paged_attn_kernel<E, D, 8, 1>, 8);
-  } else if (waves == 1) {
+    if constexpr (paged_pairs(D, E::CB)) {
+      if constexpr (paged_eight(D, E::CB, 2)) {
+        if (a.waves == 8) launch(paged_attn_kernel<E, D, 8, 2>, 8);
+      }
+      if (a.waves != 8) launch(paged_attn_kernel<E, D, 4, 2>, 4);
+    }
+  } else if (a.waves == 8) {
+    if constexpr (paged_eight(D, E::CB, 1)) launch(paged_attn_kernel<E, D, 8, 1>, 8);
+  } else if (a.waves == 1) {
     launch(paged_attn_kernel<E, D, 1, 1>, 1);
   } else {
     launch(paged_attn_kernel<E, D, 4, 1>, 4);
