@@ -70,15 +70,16 @@ int status(hipError_t e) { return e == hipSuccess ? FA_OK : FA_ERR_LAUNCH; }
 // bound is what the longest can be.  Times in us, whole / split, with 8 KV heads and D = 64 (4 and D = 128):
 //   bf16: 1 sequence of 1001 tokens 7.9 / 9.1, of 1500 9.4 / 9.1, of 2048 11.3 / 9.2; 4 of 2048 11.4 / 10.0;
 //     16 (128 workgroups) of 1500 11.7 / 16.3, of 2048 14.4 / 19.0; 64 (512 workgroups) of 2048 43.9 / 48.1, of 4096 97 / 85
-//   bf16 D = 128: 1 of 600 9.4 / 9.3, of 1000 12.6 / 9.5; 16 (64 workgroups) of 1000 13.4 / 16.0, of 2000 22.6 / 23.2
-//   e4m3 D = 128: 1 of 600 8.0 / 9.2, of 1000 10.4 / 9.3; 16 (64 workgroups) of 1000 10.8 / 11.2, of 1500 14.0 / 12.8
-//   float32: 1 of 600 12.6 / 10.0 (the lines cross at about 380); 16 (128 workgroups) of 600 14.0 / 17.6, of 1000 19.6 / 20.0;
-//     D = 128: 1 of 600 21.6 / 12.4
+//   bf16 D = 128: 1 of 600 9.4 / 9.3, of 1000 12.6 / 9.5; 16 (64 workgroups) of 700 10.6 / 14.9, of 1000 13.4 / 16.0
+//   e4m3: 8 (64 workgroups) of 1500 10.2 / 11.4, of 2000 12.2 / 11.4; 16 of 2000 12.9 / 14.5
+//   e4m3 D = 128: 1 of 600 8.0 / 9.2, of 1000 10.4 / 9.3; 16 (64 workgroups) of 1000 10.8 / 11.6, of 1500 14.1 / 13.2
+//   float32: 1 of 600 12.6 / 10.0 (the lines cross at about 380); 8 (64 workgroups) of 500 11.2 / 10.7; 16 of 500 11.9 / 13.3
+//   float32 D = 128: 1 of 600 21.6 / 12.4; 16 (64 workgroups) of 400 18.8 / 14.2
 //   64 heads over one: 1 of 600 8.7 / 10.8, of 1000 11.0 / 10.9; 16 of 1000 11.4 / 12.2, of 1500 14.1 / 13.7
 int whole_keys(int D, int cache_bytes) {
-  return cache_bytes == 4 ? 256 : D * cache_bytes > 128 ? 512 : D > 64 ? 768 : 1024;
+  return cache_bytes == 4 ? (D > 64 ? 128 : 256) : D * cache_bytes > 128 ? 512 : D > 64 ? 768 : 1024;
 }
-constexpr int kManyWgs = 128;
+constexpr int kManyWgs = 64;
 // Whole sequences are taken by 8 waves while there are at most as many workgroups as compute units (1 sequence of 1001
 // tokens: 9.2 us with 4 waves, 7.9 with 8; but 64 of 256: 7.4 and 9.5), and by a wave each where there are kSingleWgs of at
 // most kSingleUnits units (256 sliding-layer sequences 17.7 us with 4 waves, 14.2 with one; 1024 of them 78 and 59).
