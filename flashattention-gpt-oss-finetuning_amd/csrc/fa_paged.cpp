@@ -281,8 +281,8 @@ int fa_paged_evict(const fa_paged_evict_params* p, void* workspace, size_t works
   if (!workspace || !aligned(workspace, 256) || workspace_bytes < fa_paged_evict_workspace_bytes(c.batch, c.heads_kv, p->keep, int32_t(tokens)))
     return FA_ERR_WORKSPACE;
   const int row = c.head_dim * elem_bytes(c.dtype);
-  // workgroups of the launches: 1024 threads a chunk, and one for 1024 pieces of 16 bytes of kept entries
-  const int64_t heads = int64_t(c.batch) * c.heads_kv, chunk = 1024 / (row / 16);
+  // workgroups of the launches: 1024 threads a chunk, and one for each kGatherPieces of kept entries
+  const int64_t heads = int64_t(c.batch) * c.heads_kv, chunk = fa::kGatherPieces / (row / 16);
   const EvictRoom room = evict_room(heads, p->keep, tokens);
   if (!fa::grid_fits(heads * room.chunks, 1024) || !fa::grid_fits(heads * ((p->keep + chunk - 1) / chunk))) return FA_ERR_OVERFLOW;
   fa::EvictArgs a{};

@@ -65,6 +65,8 @@ struct PagedAttnArgs {
   float* logits;          // with sums: [Hkv][B][max_units][G][kPagedUnit] (log2 domain)
 };
 
+constexpr int kGatherPieces = 512;  // 16-byte pieces of K, and of V, that a workgroup of the gather moves
+
 struct EvictArgs {
   PagedCache c;
   const float* sums;

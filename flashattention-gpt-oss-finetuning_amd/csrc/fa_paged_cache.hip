@@ -13,7 +13,7 @@
 // 10.9 us, barriers and dependent steps on 64 of 256 compute units; one of 131071: four launches, 29 us in all.
 // paged_gather_kernel.  Entry r of those kept goes to position r on the pages of the new table.  Those are other pages
 // than the old ones, so no entry is read after it is overwritten and all are copied at once: 2048 entries of 8 sequences
-// (66 MB moved) 15.6 us, 4.2 TB/s, a large copy's rate being 4.9.
+// (66 MB moved) 13.6 us, 4.8 TB/s, a large copy's rate being 4.9.
 #include <hip/hip_runtime.h>
 
 #include "../../include/fa_gfx950.h"
@@ -339,8 +339,9 @@ __global__ __launch_bounds__(kSelectThreads) void paged_select_kernel(const Evic
   write_kept(sh, t, first, n, m, prefix, need, fixed + prior, equal, a.kept + int64_t(row) * a.keep, y);
 }
 
-// Entries of a workgroup: kThreads / pieces a round.
-constexpr int kGatherRounds = 4;
+// A workgroup has kThreads / pieces entries a round.  Rounds of 1 / 2 / 4 / 8: 15.7 / 13.6 / 15.6 / 18.4 us for 8 sequences, 17.2 / 16.6 /
+// 17.9 / 21.0 for one of 16384 kept entries: the look-ups of some workgroups hide behind the copies of others.
+constexpr int kGatherRounds = kGatherPieces / kThreads;
 
 template <int PIECES>
 __global__ __launch_bounds__(kThreads) void paged_gather_kernel(const EvictArgs a, int chunks) {
