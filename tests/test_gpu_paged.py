@@ -683,3 +683,25 @@ def test_inference_mode(fa, gpu):
         nt = torch.arange(c["used"], c["used"] + 2, dtype=torch.int32, device=gpu).view(2, 1)
         left, new = fa.paged_evict(kp, vp, t, lens, sums, 16, nt)
         assert left.tolist() == [16, 9] and float(sums.sum()) > 0
+
+
+def test_pools_of_different_layouts_and_narrow_sums(fa, gpu):
+    """K pages with the heads first, V pages as half of a fused pool with the slots first; sums as wide as max_seqlen."""
+    c = make(95, "bf16", "bf16", 64, 8, 2, 16, "hnd", (700, 33, 1300), nan=False)
+    P = c["kp"].shape[0]
+    fused = torch.zeros(P, 16, 2, 2, 64, dtype=torch.bfloat16, device=gpu)  # [pages, slots, K/V, heads, D]
+    vp = fused[:, :, 1].transpose(1, 2)
+    vp.copy_(c["vp"])
+    kp, t, lens = c["kp"].to(gpu), c["table"].to(gpu), c["lens"].to(gpu)
+    w = torch.rand(2, 3, 1500, generator=c["g"]).to(gpu)[:, :, 100:1400].transpose(0, 1)  # [B, Hkv, 1300], unaligned
+    w0 = w.clone()
+    ref, mag, ref_sums = oracle.attention(c["q"], c["kp"], c["vp"], c["table"], c["lens"], 1250, 7, sums=torch.zeros(3, 2, 1312))
+    o = fa.paged_attention(c["q"].to(gpu), kp, vp, t, lens, 1250, 7, max_seqlen=1300, weight_sums=w)
+    check_attention(o, c, ref, mag, "bf16", 64, 1300, 0.125, 1250, 7)
+    assert torch.allclose((w - w0).cpu().double(), ref_sums[..., :1300], atol=1e-5)
+    x = torch.randn(3, 2, 64, generator=c["g"]).to(torch.bfloat16)
+    want = oracle.append(x, x, c["kp"], c["vp"], c["table"], c["lens"])
+    fa.paged_append(x.to(gpu), x.to(gpu), kp, vp, t, lens)
+    same(kp, want[0])
+    same(vp, want[1])
+    assert not fused[:, :, 0].any()
