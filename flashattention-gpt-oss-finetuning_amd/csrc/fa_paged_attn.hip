@@ -30,7 +30,7 @@
 // sizes the host knows.  Pieces that are no whole sequence leave (maximum, sum, o) in the workspace, and
 // paged_finish_kernel joins them.
 //
-// Measured (D = 64, bf16, 8 heads a group; rocprofv3): 32 ragged sequences, 261 MB of K and V, 49 to 51 us, 5.2 TB/s; four of up to 128K
+// Measured (D = 64, bf16, 8 heads a group; rocprofv3): 32 ragged sequences, 261 MB of K and V, 48 to 50 us, 5.3 TB/s; four of up to 128K
 // tokens, 876 MB, 142 us with the heads before the slots in a page, 6.2 TB/s, and 157 with the slots first.  The
 // counters show 261 and 877 MB read: every entry once.  A plain kernel that only reads reaches 6.2 TB/s, 7.1 with loads marked as read
 // once.  Without the products and the softmax (loads only) the kernel took the same time to 3%.
@@ -62,31 +62,42 @@ __device__ __forceinline__ int units_of(const PagedAttnArgs& a, int b) {
   return b < a.c.B ? paged_units(visible(seq_len(a.c, b), a.W, a.S).count) : 0;
 }
 
-// Units of all sequences (every lane of the wave calls).
-__device__ __forceinline__ int total_units(const PagedAttnArgs& a) {
-  int n = 0;
+// The units of the sequences, 64 at a time over the lanes of a wave, all of which call.
+struct Units {
+  int n, upto;  // of this lane's sequence, and of the 64 up to it
+  __device__ __forceinline__ int all() const { return __builtin_amdgcn_readfirstlane(__shfl(upto, 63)); }
+};
+__device__ __forceinline__ Units units_from(const PagedAttnArgs& a, int b0) {
+  const int lane = threadIdx.x & 63, n = units_of(a, b0 + lane);
+  return Units{n, wave_prefix(n, lane)};
+}
+
+// Units of all sequences; the first 64 sequences' are in `first`.
+__device__ __forceinline__ int total_units(const PagedAttnArgs& a, const Units& first) {
+  if (a.c.B <= 64) return first.all();
+  int n = first.n;
 #pragma unroll 4
-  for (int b0 = 0; b0 < a.c.B; b0 += 64) n += units_of(a, b0 + (threadIdx.x & 63));
+  for (int b0 = 64; b0 < a.c.B; b0 += 64) n += units_of(a, b0 + (threadIdx.x & 63));
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) n += __shfl_xor(n, o);
   return __builtin_amdgcn_readfirstlane(n);
 }
 
 // The sequence that holds unit u < total, and its first unit.
-__device__ __forceinline__ void find_unit(const PagedAttnArgs& a, int u, int& b, int& start) {
-  const int lane = threadIdx.x & 63;
+__device__ __forceinline__ void find_unit(const PagedAttnArgs& a, Units x, int u, int& b, int& start) {
   int base = 0;
-  for (int b0 = 0; b0 < a.c.B; b0 += 64) {
-    const int n = units_of(a, b0 + lane);
-    const int x = wave_prefix(n, lane);
-    const unsigned long long m = __ballot(base + x > u);
+  for (int b0 = 0;;) {
+    const unsigned long long m = __ballot(base + x.upto > u);
     if (m) {
       const int l = __builtin_amdgcn_readfirstlane(__ffsll(m) - 1);
       b = b0 + l;
-      start = base + __builtin_amdgcn_readfirstlane(__shfl(x - n, l));
+      start = base + __builtin_amdgcn_readfirstlane(__shfl(x.upto - x.n, l));
       return;
     }
-    base += __builtin_amdgcn_readfirstlane(__shfl(x, 63));
+    base += x.all();
+    b0 += 64;
+    if (b0 >= a.c.B) break;
+    x = units_from(a, b0);
   }
   b = 0;  // (not reached: u < total)
   start = 0;
@@ -437,13 +448,14 @@ __global__ __launch_bounds__(64 * WAVES) void paged_attn_kernel(const PagedAttnA
     start = u = 0;
     end = 1;
   } else {
-    const int total = total_units(a);
+    const Units first = units_from(a, 0);
+    const int total = total_units(a, first);
     per = units_per_part(total, a.parts, a.least);
     once = total > a.keep_units;
     if (int64_t(part) * per >= total) return;
     u = part * per;
     end = imin(total, u + per);
-    find_unit(a, u, b, start);
+    find_unit(a, first, u, b, start);
   }
 
   Wave<E, D, RT> w;
