@@ -3,8 +3,8 @@
 //
 // paged_append_kernel.  Row i of sequence b's n new rows goes to position lens[b] - n + i.  A wave takes a row: it finds the
 // row's sequence by one ballot over cu_seqlens and the page once, then its lanes copy the 16-byte pieces of
-// every head's K and V: a prompt of 16384 rows (67 MB moved) 13 us, 5.1 TB/s; into e4m3 pages, D = 128 (35 MB), 10.6; a decoding
-// step of 64 rows 3.4, all latency.  e4m3 pages get the codes of clamp(x * fl32(1 / descale), -448, 448), as quantize_fp8's.
+// every head's K and V: a prompt of 16384 rows (67 MB moved) 12.7 us, 5.3 TB/s; into e4m3 pages, D = 128 (35 MB), 10.5; a
+// decoding step of 64 rows 2.8, all latency.  Two rows a wave gained nothing (12.6, 11.2, 4.0).  e4m3 pages get the codes of clamp(x * fl32(1 / descale), -448, 448), as quantize_fp8's.
 //
 // paged_select_kernel.  Of a (sequence, KV head)'s n entries the first S and the last R stay, and of the others the
 // keep - S - R of the largest weight, the lower index first among equals (NaN counts as the largest).  The weights are
@@ -102,16 +102,19 @@ __global__ __launch_bounds__(kThreads) void paged_append_kernel(const AppendArgs
   const int pi = page_of(a.c.div, int(pos)), slot = int(pos) - pi * a.c.page_size;
   const int page = a.c.table[int64_t(b) * a.c.table_stride + pi];
   if (page < 0 || page >= a.c.pages) return;
-  const int n = a.c.Hkv * PP;
-  for (int i = lane; i < 2 * n; i += 64) {
-    const bool is_v = i >= n;
-    const int p = is_v ? i - n : i, h = p / PP, piece = p % PP;
-    const u32x4 x = is_v ? ld16(a.v + int64_t(h) * a.sv[0] + int64_t(row) * a.sv[1] + 16 * piece)
-                         : ld16(a.k + int64_t(h) * a.sk[0] + int64_t(row) * a.sk[1] + 16 * piece);
-    uint8_t* d = is_v ? a.c.v + int64_t(page) * a.c.sv[0] + int64_t(h) * a.c.sv[1] + int64_t(slot) * a.c.sv[2]
-                      : a.c.k + int64_t(page) * a.c.sk[0] + int64_t(h) * a.c.sk[1] + int64_t(slot) * a.c.sk[2];
-    if constexpr (Q) *reinterpret_cast<u32x2*>(d + 8 * piece) = encode8<T>(x, is_v ? a.v_inv : a.k_inv);
-    else st16(d + 16 * piece, x);
+  uint8_t* dk = a.c.k + int64_t(page) * a.c.sk[0] + int64_t(slot) * a.c.sk[2];
+  uint8_t* dv = a.c.v + int64_t(page) * a.c.sv[0] + int64_t(slot) * a.c.sv[2];
+  for (int i = lane; i < a.c.Hkv * PP; i += 64) {
+    const int h = i / PP, piece = i % PP;
+    const u32x4 k = ld16(a.k + int64_t(h) * a.sk[0] + int64_t(row) * a.sk[1] + 16 * piece);
+    const u32x4 v = ld16(a.v + int64_t(h) * a.sv[0] + int64_t(row) * a.sv[1] + 16 * piece);
+    if constexpr (Q) {
+      *reinterpret_cast<u32x2*>(dk + int64_t(h) * a.c.sk[1] + 8 * piece) = encode8<T>(k, a.k_inv);
+      *reinterpret_cast<u32x2*>(dv + int64_t(h) * a.c.sv[1] + 8 * piece) = encode8<T>(v, a.v_inv);
+    } else {
+      st16(dk + int64_t(h) * a.c.sk[1] + 16 * piece, k);
+      st16(dv + int64_t(h) * a.c.sv[1] + 16 * piece, v);
+    }
   }
 }
 

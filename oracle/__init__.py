@@ -13,6 +13,8 @@ Contents
                restatement of HF transformers' eager GPT-OSS attention; variable-length
                (packed) batches as independent sequences, and the packed batch's
                block-diagonal mask.
+  paged.py  -- the paged key-value cache in float64: appending rows, attention of one new token a
+               sequence, eviction by accumulated weight.
   loops.py  -- pure-Python double loop over (q, k) for tiny shapes: a second, independent
                statement of the mask and of the forward.
 
@@ -26,6 +28,8 @@ logit (an independent statement of "a logit in the denominator without a value")
 installed transformers package's own eager_attention_forward, against the no-sink oracle for a
 sink of -inf, and by gradcheck for the sink gradient.  The variable-length oracle is pinned
 against one SDPA call over the whole packed batch with the block-diagonal mask (and autograd
-for the gradients), and against single-sequence batches of the fixed-length oracle.  The
+for the gradients), and against single-sequence batches of the fixed-length oracle.  The paged
+oracle is pinned (tests/test_oracle_paged.py) against SDPA over the gathered keys with an explicit
+mask, plain indexing, and a stable sort for eviction.  The
 reference ships no golden vectors of its own (it has no test suite).
 """
