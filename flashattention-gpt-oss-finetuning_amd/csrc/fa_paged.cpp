@@ -89,13 +89,22 @@ constexpr int kSingleWgs = 1024, kSingleUnits = 2;
 // quarter of the bytes: 137 us with 2, 113 with 3 (537 MB).  A unit more a workgroup costs a short call more than its piece
 // does (1 sequence of 2048 tokens: 10.3 us with at least two units each, 9.8 with one).
 constexpr int kPartsPerCu = 2, kPartsNarrow = 3, kLeastUnits = 1;
+// Where a page has its slots before its heads, the workgroups of a part's KV heads read neighbouring pieces of the same rows, and
+// twice as many and shorter runs keep them closer together: 876 MB 152 us with 2 a compute unit, 145 with 4; but 261 MB 52.7
+// and 52.6, 71 MB 17.8 and 20.3.  So the second half of the parts is used above kManyBytes of K and V.
+constexpr int64_t kManyBytes = int64_t(384) << 20;
 // Loads of a call that reads more than this are marked as read once, so that they do not run through the 256 MB last-level
 // cache: 537 MB take 84 us so and 103 otherwise, 261 MB 49 and 54.  Below, the next step finds the keys there: three caches of 71 MB
 // in turn take 17.4 us each, 19.3 with marked loads.
 constexpr int64_t kKeepBytes = int64_t(96) << 20;
 
+// K and V bytes of a unit of keys, all KV heads.
+int64_t unit_bytes(const fa_paged_cache& c) {
+  return int64_t(fa::kPagedUnit) * 2 * c.head_dim * elem_bytes(c.dtype) * c.heads_kv;
+}
+
 struct Plan {
-  int max_units, row_tiles, rt, parts;
+  int max_units, row_tiles, rt, parts, few, many_units;
   size_t starts, part_o, part_ml, norm, logits;  // bytes
   size_t bytes() const { return std::max<size_t>(256, starts + part_o + part_ml + norm + logits); }
 };
@@ -128,12 +137,15 @@ int plan(const fa_paged_attention_params* p, Plan* r) {
   r->rt = r->row_tiles > 1 && fa::paged_pairs(c.head_dim, elem_bytes(c.dtype)) ? 2 : 1;
   const int64_t streams = int64_t(c.heads_kv) * ((r->row_tiles + r->rt - 1) / r->rt), units = int64_t(c.batch) * r->max_units;
   if (units >= (int64_t(1) << 30) || !fa::grid_fits(std::max(streams, int64_t(p->heads_q)) * c.batch)) return FA_ERR_OVERFLOW;
-  r->parts = 0;
+  r->parts = r->few = r->many_units = 0;
   if (most > whole_keys(c.head_dim, elem_bytes(c.dtype)) * (streams * c.batch >= kManyWgs ? 2 : 1)) {
     const int64_t want = std::max<int64_t>(1, int64_t(c.head_dim * elem_bytes(c.dtype) <= 32 ? kPartsNarrow : kPartsPerCu) * fa::device_cus() / streams);
     // (whole rounds of the 8 XCDs: the workgroups of a part, which read the same or neighbouring entries, then share an L2; pages
     // with the slots before the heads, 876 MB: 166 us with a KV head an XCD, 158 so)
     r->parts = int((std::min(want, (units + kLeastUnits - 1) / kLeastUnits) + 7) / 8 * 8);
+    r->few = r->parts;
+    r->many_units = int(std::min<int64_t>(kManyBytes / unit_bytes(c), INT32_MAX));
+    if (c.k_stride[1] < c.k_stride[2] && units > r->many_units) r->parts *= 2;
     if (!fa::grid_fits(streams * r->parts)) return FA_ERR_OVERFLOW;
   }
   const size_t slots = size_t(c.heads_kv) * r->row_tiles * r->parts * 2;
@@ -241,12 +253,14 @@ int fa_paged_attention(const fa_paged_attention_params* p, void* workspace, size
   a.oscale = q8 ? float(c.v_descale) : 1.f;
   a.max_units = r.max_units;
   a.parts = r.parts;
+  a.few = r.few;
+  a.many_units = r.many_units;
   a.least = kLeastUnits;
   const int64_t wgs = int64_t(c.heads_kv) * ((r.row_tiles + r.rt - 1) / r.rt) * c.batch;
   if (r.parts) a.waves = 4;
   else if (wgs <= fa::device_cus() && fa::paged_eight(c.head_dim, elem_bytes(c.dtype), r.rt)) a.waves = 8;
   else a.waves = r.rt == 1 && wgs >= kSingleWgs && r.max_units <= kSingleUnits ? 1 : 4;
-  a.keep_units = int(std::min<int64_t>(kKeepBytes / (int64_t(fa::kPagedUnit) * 2 * c.head_dim * elem_bytes(c.dtype) * c.heads_kv), INT32_MAX));
+  a.keep_units = int(std::min<int64_t>(kKeepBytes / unit_bytes(c), INT32_MAX));
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   a.starts = reinterpret_cast<int*>(ws);
   a.part_o = reinterpret_cast<float*>(ws += r.starts);

@@ -54,6 +54,7 @@ struct PagedAttnArgs {
   int max_units;          // units of a sequence of max_len tokens
   // split calls: the runs a (KV head, row tile) is cut into, 0 where every workgroup takes a whole sequence
   int parts, least;
+  int few, many_units;    // calls of at most many_units units use the first `few` of the parts only
   int waves;              // of a workgroup: 1 (only with rt = 1), 4 or 8 (paged_eight)
   int rt;                 // tiles of heads that a workgroup takes: 1, or 2 (paged_pairs)
   int keep_units;         // calls that read more units a KV head than this mark their loads as read once

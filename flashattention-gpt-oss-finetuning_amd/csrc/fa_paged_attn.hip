@@ -31,9 +31,9 @@
 // paged_finish_kernel joins them.
 //
 // Measured (D = 64, bf16, 8 heads a group; rocprofv3): 32 ragged sequences, 261 MB of K and V, 48 to 50 us, 5.3 TB/s; four of up to 128K
-// tokens, 876 MB, 142 us with the heads before the slots in a page, 6.2 TB/s, and 157 with the slots first.  The
+// tokens, 876 MB, 143 us, 6.1 TB/s, with the heads before the slots in a page and with the slots first.  The
 // counters show 261 and 877 MB read: every entry once.  A plain kernel that only reads reaches 6.2 TB/s, 7.1 with loads marked as read
-// once.  Without the products and the softmax (loads only) the kernel took the same time to 3%.
+// once.  Without the products and the softmax (loads only) the kernel took the same time to 5%.
 // What is left of a small call is latency: lens, table, K, four tiles, the waves' sums: one sliding-layer step 5.3 us.
 #include <hip/hip_runtime.h>
 
@@ -450,7 +450,7 @@ __global__ __launch_bounds__(64 * WAVES) void paged_attn_kernel(const PagedAttnA
   } else {
     const Units first = units_from(a, 0);
     const int total = total_units(a, first);
-    per = units_per_part(total, a.parts, a.least);
+    per = units_per_part(total, total > a.many_units ? a.parts : a.few, a.least);
     once = total > a.keep_units;
     if (int64_t(part) * per >= total) return;
     u = part * per;

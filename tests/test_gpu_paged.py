@@ -170,10 +170,10 @@ def test_many_short_sequences(fa, gpu, B, Hq, Hkv, D, cache, W):
     check_attention(o, c, ref, mag, dtype, D, 260, 1 / math.sqrt(D), W, 3 if W else 0)
 
 
-def test_large_cache(fa, gpu):
-    """270 MB of K and V, so that loads are marked as read once, in two layouts, with weights."""
-    B, Hq, Hkv, D, page = 3, 16, 2, 64, 64
-    lens = [300001, 70000, 140000]
+@pytest.mark.parametrize("lens", [[300001, 70000, 140000], [610001, 200000]])
+def test_large_cache(fa, gpu, lens):
+    """260 and 415 MB of K and V, so that loads are marked as read once and more workgroups used, in two layouts, with weights."""
+    B, Hq, Hkv, D, page = len(lens), 16, 2, 64, 64
     g = torch.Generator(device=gpu).manual_seed(5)
     used = [-(-n // page) for n in lens]
     P = sum(used)
