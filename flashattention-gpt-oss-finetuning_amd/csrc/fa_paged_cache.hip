@@ -346,20 +346,22 @@ __global__ __launch_bounds__(kSelectThreads) void paged_select_kernel(const Evic
 // 17.9 / 21.0 for one of 16384 kept entries: the look-ups of some workgroups hide behind the copies of others.
 constexpr int kGatherRounds = kGatherPieces / kThreads;
 
-template <int PIECES>
+// The entries are taken in the order of the pages they go to: a head's one after the other, or (ACROSS) an entry of every
+// head before the next ones.
+template <int PIECES, bool ACROSS>
 __global__ __launch_bounds__(kThreads) void paged_gather_kernel(const EvictArgs a, int chunks) {
   constexpr int ROWS = kThreads / PIECES;
-  const int chunk = blockIdx.x % chunks, s = blockIdx.x / chunks, hkv = s % a.c.Hkv, b = s / a.c.Hkv;
+  const int chunk = blockIdx.x % chunks, s = blockIdx.x / chunks, b = ACROSS ? s : s / a.c.Hkv;
   const int n = seq_len(a.c, b), m = imin(n, a.keep);
-  const int* kept = a.kept + int64_t(s) * a.keep;
   const int* from = a.c.table + int64_t(b) * a.c.table_stride;
   const int* to = a.new_table + int64_t(b) * a.new_table_stride;
   const int piece = threadIdx.x % PIECES;
 #pragma unroll
   for (int x = 0; x < kGatherRounds; ++x) {
-    const int r = (chunk * kGatherRounds + x) * ROWS + int(threadIdx.x) / PIECES;
+    const int e = (chunk * kGatherRounds + x) * ROWS + int(threadIdx.x) / PIECES;
+    const int r = ACROSS ? e / a.c.Hkv : e, hkv = ACROSS ? e % a.c.Hkv : s % a.c.Hkv;
     if (r >= m) continue;
-    const int i = kept[r];
+    const int i = a.kept[(int64_t(b) * a.c.Hkv + hkv) * a.keep + r];
     if (i < 0 || i >= n) continue;  // (never, unless lens or weights change under the running call)
     const int pi = page_of(a.c.div, i), slot = i - pi * a.c.page_size, qi = page_of(a.c.div, r), new_slot = r - qi * a.c.page_size;
     const int page = from[pi], new_page = to[qi];
@@ -373,8 +375,15 @@ __global__ __launch_bounds__(kThreads) void paged_gather_kernel(const EvictArgs 
 
 template <int PIECES>
 hipError_t gather(const EvictArgs& a, hipStream_t s) {
-  const int rows = kThreads / PIECES * kGatherRounds, chunks = (a.keep + rows - 1) / rows;
-  hipLaunchKernelGGL(paged_gather_kernel<PIECES>, dim3(unsigned(chunks) * unsigned(a.c.B * a.c.Hkv)), dim3(kThreads), 0, s, a, chunks);
+  const int rows = kThreads / PIECES * kGatherRounds;
+  const int64_t entries = int64_t(a.keep) * a.c.Hkv;
+  if (a.c.sk[1] < a.c.sk[2] && entries < (int64_t(1) << 30)) {
+    const int chunks = int((entries + rows - 1) / rows);
+    hipLaunchKernelGGL((paged_gather_kernel<PIECES, true>), dim3(unsigned(chunks) * unsigned(a.c.B)), dim3(kThreads), 0, s, a, chunks);
+  } else {
+    const int chunks = (a.keep + rows - 1) / rows;
+    hipLaunchKernelGGL((paged_gather_kernel<PIECES, false>), dim3(unsigned(chunks) * unsigned(a.c.B * a.c.Hkv)), dim3(kThreads), 0, s, a, chunks);
+  }
   return hipGetLastError();
 }
 
