@@ -162,8 +162,16 @@ int plan(const fa_paged_attention_params* p, Plan* r) {
   return FA_OK;
 }
 
-// Weights that a thread of the selection holds where one workgroup a (sequence, KV head) does not hold them all.
-constexpr int kSplitEach = 8;
+// Weights that a thread of the selection holds.  Up to 16384 entries one workgroup takes a (sequence, KV head) in one launch.  More
+// are cut into chunks: the smallest that leave a CU one workgroup, for each reads the counts of all chunks of its head.  With 4 / 8 /
+// 16 (whole evictions): 8 heads of 32000 entries 29 / 34 / 40 us, 8 of 131071 42 / 42 / 48, 64 of 50000 116 / 82 / 65, 128 of 32000
+// 104 / 80 / 66, 240 of 50000 372 / 276 / 241.
+int select_each(int64_t heads, int64_t tokens) {
+  if (tokens <= 16384) return tokens <= 4096 ? 4 : tokens <= 8192 ? 8 : 16;
+  for (int each = 4; each < 16; each *= 2)
+    if (heads * ((tokens + 1024 * each - 1) / (1024 * each)) <= 256) return each;
+  return 16;
+}
 
 // An eviction's launches and the bytes of its workspace.
 struct EvictRoom {
@@ -172,7 +180,7 @@ struct EvictRoom {
 };
 EvictRoom evict_room(int64_t heads, int32_t keep, int64_t tokens) {
   EvictRoom r{};
-  r.each = tokens <= 4096 ? 4 : tokens <= 8192 ? 8 : tokens <= 16384 ? 16 : kSplitEach;
+  r.each = select_each(heads, tokens);
   r.chunks = int((tokens + 1024 * r.each - 1) / (1024 * r.each));
   r.kept = align256(size_t(heads) * keep * sizeof(int32_t));
   if (r.chunks > 1) {

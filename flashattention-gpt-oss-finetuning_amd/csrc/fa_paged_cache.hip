@@ -346,8 +346,10 @@ __global__ __launch_bounds__(kSelectThreads) void paged_select_kernel(const Evic
 // 17.9 / 21.0 for one of 16384 kept entries: the look-ups of some workgroups hide behind the copies of others.
 constexpr int kGatherRounds = kGatherPieces / kThreads;
 
-// The entries are taken in the order of the pages they go to: a head's one after the other, or (ACROSS) an entry of every
-// head before the next ones.
+// The entries are taken in the order of the pages they go to: a head's one after the other, or (ACROSS, pages with their slots first)
+// an entry of every head before the next ones, so that a workgroup writes whole rows.  By heads / ACROSS, slots first: 153 / 87 us
+// for 15 sequences of 16 heads with D = 16 that keep 7642 entries, where an entry of one head is 32 bytes; 16.4 / 16.1 for one of
+// 16384 with D = 64.
 template <int PIECES, bool ACROSS>
 __global__ __launch_bounds__(kThreads) void paged_gather_kernel(const EvictArgs a, int chunks) {
   constexpr int ROWS = kThreads / PIECES;

@@ -366,6 +366,9 @@ EVICT = [
     ("fp16", 16, 2, 64, "nhd", (40000, 16385, 5, 20000, 16384), 3000, 4, 100),
     ("bf16", 16, 1, 16, "hnd", (40001, 33000), 20000, 17000, 0),
     ("bf16", 16, 1, 16, "hnd", (49153, 32769), 20000, 0, 17000),
+    # more (sequence, KV head) than one workgroup each fills the card with
+    ("bf16", 16, 24, 16, "nhd", (20001, 16385, 100), 3000, 1, 30),
+    ("bf16", 16, 48, 16, "hnd", (20001, 16385, 8193), 3000, 1, 30),
 ]
 
 
