@@ -31,7 +31,7 @@ int check_cache(const fa_paged_cache& c) {
   if (!aligned(c.k, 16) || !aligned(c.v, 16) || !aligned(c.table, 4) || !aligned(c.lens, 4) || c.table_stride < 0 ||
       !strides_ok(c.k_stride, 3, eb) || !strides_ok(c.v_stride, 3, eb))
     return FA_ERR_ALIGN;
-  if (int64_t(c.table_width) * c.page_size >= fa::kPagedMaxTokens) return FA_ERR_OVERFLOW;
+  if (int64_t(c.table_width) * c.page_size >= fa::kPagedMaxTokens || c.heads_kv >= 1 << 24) return FA_ERR_OVERFLOW;
   return FA_OK;
 }
 
@@ -169,7 +169,7 @@ int plan(const fa_paged_attention_params* p, Plan* r) {
 int select_each(int64_t heads, int64_t tokens) {
   if (tokens <= 16384) return tokens <= 4096 ? 4 : tokens <= 8192 ? 8 : 16;
   for (int each = 4; each < 16; each *= 2)
-    if (heads * ((tokens + 1024 * each - 1) / (1024 * each)) <= 256) return each;
+    if ((tokens + 1024 * each - 1) / (1024 * each) <= 256 / heads) return each;
   return 16;
 }
 
@@ -294,7 +294,8 @@ int fa_paged_evict(const fa_paged_evict_params* p, void* workspace, size_t works
   if (p->keep < 1 || p->sink < 0 || p->recent < 0 || int64_t(p->sink) + p->recent > p->keep || p->sums_width < tokens ||
       p->new_table_width < 1 || int64_t(p->new_table_width) * c.page_size < p->keep)
     return FA_ERR_PAGES;
-  if (p->keep >= fa::kPagedMaxTokens) return FA_ERR_OVERFLOW;
+  const int64_t heads = int64_t(c.batch) * c.heads_kv;
+  if (p->keep >= fa::kPagedMaxTokens || !fa::grid_fits(heads)) return FA_ERR_OVERFLOW;
   if (!aligned(p->sums, 4) || !aligned(p->new_sums, 4) || !aligned(p->new_table, 4) || !aligned(p->new_lens, 4) ||
       p->new_table_stride < 0)
     return FA_ERR_ALIGN;
@@ -304,7 +305,7 @@ int fa_paged_evict(const fa_paged_evict_params* p, void* workspace, size_t works
     return FA_ERR_WORKSPACE;
   const int row = c.head_dim * elem_bytes(c.dtype);
   // workgroups of the launches: 1024 threads a chunk, and one for each kGatherPieces of kept entries
-  const int64_t heads = int64_t(c.batch) * c.heads_kv, chunk = fa::kGatherPieces / (row / 16);
+  const int64_t chunk = fa::kGatherPieces / (row / 16);
   const EvictRoom room = evict_room(heads, p->keep, tokens);
   if (!fa::grid_fits(heads * room.chunks, 1024) || !fa::grid_fits(heads * ((p->keep + chunk - 1) / chunk))) return FA_ERR_OVERFLOW;
   fa::EvictArgs a{};

@@ -152,6 +152,18 @@ def test_evict_workspace():
         assert L.fa_paged_evict(ctypes.byref(_evict()), ws, n, None) == _code("WORKSPACE")
 
 
+def test_sizes_whose_products_pass_64_bits():
+    L, many = _lib.lib(), dict(batch=1 << 28, heads_kv=1 << 28, k_stride=(0, 0, 64), v_stride=(0, 0, 64))
+    p = _attn(cache=_cache(**many), heads_q=1 << 28)
+    assert L.fa_paged_attention(ctypes.byref(p), FAKE, 1 << 40, None) == _code("OVERFLOW")
+    assert L.fa_paged_evict(ctypes.byref(_evict(_cache(**many))), FAKE, 1 << 40, None) == _code("OVERFLOW")
+    # heads_kv within its own limit: batch * heads * 256 threads is 2^60 and more, the kept entries' bytes too
+    q = _cache(**{**many, "heads_kv": 1 << 23, "batch": 1 << 30})
+    p = _attn(cache=q, heads_q=1 << 30)
+    assert L.fa_paged_attention(ctypes.byref(p), FAKE, 1 << 40, None) == _code("OVERFLOW")
+    assert L.fa_paged_evict(ctypes.byref(_evict(q)), FAKE, 1 << 40, None) == _code("OVERFLOW")
+
+
 def test_struct_layouts_match_header():
     src = ('#include "fa_gfx950.h"\n#include <stdio.h>\n#include <stddef.h>\nint main(void){printf("%zu %zu %zu %zu %zu %zu\\n",'
            "sizeof(fa_paged_cache), sizeof(fa_paged_attention_params), sizeof(fa_paged_evict_params), offsetof(fa_paged_cache, k_descale),"
