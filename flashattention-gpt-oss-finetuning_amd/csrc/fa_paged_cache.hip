@@ -275,11 +275,13 @@ __device__ __forceinline__ void write_kept(SelectShared& sh, const Entries<EACH>
 // one launch does everything.  Otherwise launch `stage` = 0, 1, 2 leaves the chunks' counts of digit `stage` in the
 // workspace, from which every workgroup of the next launch finds the digit for itself, and launch 3 writes: no
 // atomic in memory, nothing to clear, and nobody waits for another workgroup.
+// The chunks of a head are as many workgroups apart as there are heads: with a multiple of 8 of them they run on one XCD and share the
+// counts in its L2 (8 heads of 131071 entries 42.7 -> 41.3 us, of 32000 29.4 -> 26.8).
 template <int EACH>
 __global__ __launch_bounds__(kSelectThreads) void paged_select_kernel(const EvictArgs a, int stage) {
   constexpr int kChunk = EACH * kSelectThreads;
   __shared__ SelectShared sh;
-  const int chunk = blockIdx.x % a.chunks, row = blockIdx.x / a.chunks, hkv = row % a.c.Hkv, b = row / a.c.Hkv;
+  const int rows = a.c.B * a.c.Hkv, chunk = blockIdx.x / rows, row = blockIdx.x % rows, hkv = row % a.c.Hkv, b = row / a.c.Hkv;
   const int tid = threadIdx.x, first = chunk * kChunk;
   const bool last = a.chunks == 1 || stage == kDigits;
   Entries<EACH> t;
