@@ -299,24 +299,13 @@ def _plain_evict(s):
     return s["k_pages"], s["v_pages"], left.to(torch.int32), new
 
 
-_package = None
-
-
-def _fa():
-    """The package, looked up once, as a program imports it once."""
-    global _package
-    if _package is None:
-        _package = importlib.import_module(PKG)
-    return _package
-
-
 def run(state):
     s = state
     case = s["case"]
     op = case["op"]
     if not own:
         return (_plain_append if op == "append" else _plain_attend if op == "attend" else _plain_evict)(s)
-    fa = _fa()
+    fa = importlib.import_module(PKG)
     if op == "append":
         fa.paged_append(s["k"], s["v"], s["k_pages"], s["v_pages"], s["table"], s["lens"], cu_seqlens=s["cu"],
                         descale=s["descale"])
