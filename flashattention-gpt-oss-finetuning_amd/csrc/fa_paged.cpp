@@ -184,7 +184,7 @@ EvictRoom evict_room(int64_t heads, int32_t keep, int64_t tokens) {
   r.chunks = int((tokens + 1024 * r.each - 1) / (1024 * r.each));
   r.kept = align256(size_t(heads) * keep * sizeof(int32_t));
   if (r.chunks > 1) {
-    r.state = align256(size_t(heads) * r.chunks * 3 * sizeof(int32_t));
+    r.state = align256(size_t(heads) * r.chunks * fa::kSelectState * sizeof(int32_t));
     r.counts = align256(size_t(heads) * r.chunks * 3 * 2048 * sizeof(uint16_t));
   }
   return r;

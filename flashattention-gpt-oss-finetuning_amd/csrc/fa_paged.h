@@ -68,6 +68,8 @@ struct PagedAttnArgs {
 
 constexpr int kGatherPieces = 512;  // 16-byte pieces of K, and of V, that a workgroup of the gather moves
 
+constexpr int kSelectState = 8;     // numbers that a workgroup of the selection hands on to the next launch
+
 struct EvictArgs {
   PagedCache c;
   const float* sums;
@@ -81,7 +83,7 @@ struct EvictArgs {
   int each, chunks;       // chunks of 1024 each entries, a (sequence, KV head); each is 4, 8 or 16
   // workspace
   int* kept;              // [B][Hkv][keep] entries kept, in order
-  int* state;             // with several chunks: [B][Hkv][chunks][3]
+  int* state;             // with several chunks: [B][Hkv][chunks][kSelectState]
   uint16_t* counts;       // with several chunks: [B][Hkv][3 digits][chunks][2048]
 };
 

@@ -7,7 +7,9 @@
 // decoding step of 64 rows 2.8, all latency.  Two rows a wave gained nothing (12.6, 11.2, 4.0).  e4m3 pages get the codes of clamp(x * fl32(1 / descale), -448, 448), as quantize_fp8's.
 //
 // paged_select_kernel.  Of a (sequence, KV head)'s n entries the first S and the last R stay, and of the others the
-// keep - S - R of the largest weight, the lower index first among equals (NaN counts as the largest).  The weights are
+// keep - S - R of the largest weight, the lower index first among equals (NaN counts as the largest).  Entries on no page are
+// none of the sequence's: attention masks them, and a kept one would get a place that it cannot fill.  One look over the
+// sequence's row of the table (1 us in the first launch) says whether there are any; only then are those on pages counted.  The weights are
 // mapped to unsigned numbers of the same order; three digits of them, from the top, find the smallest one that stays and
 // how many equal to it do; then the entries that stay are numbered in order.  8 sequences of up to 8192 tokens, 8 heads:
 // 10.9 us, barriers and dependent steps on 64 of 256 compute units; one of 131071: four launches, 29 us in all.
@@ -148,12 +150,14 @@ template <int EACH>
 struct Entries {
   float x[EACH];
   uint32_t u[EACH];
-  uint32_t open;  // bit e: the entry may be chosen; the others stay, or are none
+  uint32_t live;  // bit e: it is an entry of the sequence, on a page
+  uint32_t open;  // bit e: of these, it may be chosen; the others stay
 };
 
 struct SelectShared {
   uint32_t hist[kBins];
   int wave[2][kSelectWaves];
+  int gaps[kSelectWaves], live[4][kSelectWaves];
   uint32_t digit;
   int need, prior, equal;
 };
@@ -175,22 +179,75 @@ __device__ __forceinline__ void read_entries(Entries<EACH>& t, const float* x, i
     for (int e = 0; e < EACH; ++e) t.x[e] = i0 + e < width ? x[i0 + e] : 0.f;
   }
 }
+
+// How many of a sequence's positions before some are on a page.
+struct Live {
+  int gaps;                // is there a page of the sequence that the table does not name?
+  int all, lo, hi, first;  // before its end n, before `lo`, `hi` and `first`, each of them at most n
+};
+// The same in every thread; a barrier is inside.  seen: table[tid], if the table is as wide.
+__device__ __forceinline__ Live count_live(SelectShared& sh, const PagedCache& c, const int* table, int seen, int n, int lo, int hi, int first) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int pages = n > 0 ? page_of(c.div, n - 1) + 1 : 0;
+  auto named = [&](int page) { return page >= 0 && page < c.pages; };
+  bool gap = tid < pages && !named(seen);
+  for (int p = tid + kSelectThreads; p < pages; p += kSelectThreads) gap |= !named(table[p]);
+  if (const bool any = wave_any(gap); lane == 0) sh.gaps[wave] = any;
+  __syncthreads();
+  Live r{0, n, lo, hi, first};
+#pragma unroll
+  for (int w = 0; w < kSelectWaves; ++w) r.gaps |= sh.gaps[w];
+  if (!r.gaps) return r;
+  int x[4] = {0, 0, 0, 0};
+  for (int p = tid; p < pages; p += kSelectThreads) {
+    if (!named(table[p])) continue;
+    const int at = p * c.page_size;
+    auto of = [&](int end) { return imin(imax(end - at, 0), c.page_size); };
+    x[0] += of(n);
+    x[1] += of(lo);
+    x[2] += of(hi);
+    x[3] += of(first);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) x[i] += __shfl_xor(x[i], o);
+    if (lane == 0) sh.live[i][wave] = x[i];
+  }
+  __syncthreads();
+  r = Live{1, 0, 0, 0, 0};
+  for (int w = 0; w < kSelectWaves; ++w) {
+    r.all += sh.live[0][w];
+    r.lo += sh.live[1][w];
+    r.hi += sh.live[2][w];
+    r.first += sh.live[3][w];
+  }
+  return r;
+}
+
 template <int EACH>
-__device__ __forceinline__ void order_entries(Entries<EACH>& t, int first, int lo, int hi) {
+__device__ __forceinline__ void order_entries(Entries<EACH>& t, const PagedCache& c, const int* table, bool gaps, int first, int n, int lo, int hi) {
   const int i0 = first + EACH * int(threadIdx.x);
-  t.open = 0;
+  t.live = t.open = 0;
 #pragma unroll
   for (int e = 0; e < EACH; ++e) {
     t.u[e] = order_of(t.x[e]);
+    t.live |= uint32_t(i0 + e < n) << e;
     t.open |= uint32_t(i0 + e >= lo && i0 + e < hi) << e;
+  }
+  if (gaps) {
+    for (int e = 0; e < EACH && i0 + e < n; ++e) {
+      const int page = table[page_of(c.div, i0 + e)];
+      if (page < 0 || page >= c.pages) t.live &= ~(1u << e);
+    }
+    t.open &= t.live;
   }
 }
 
-// sh.hist: how many open entries whose digits above digit q are `prefix` have each value of that digit.
+// sh.hist, which is zero: how many open entries whose digits above digit q are `prefix` have each value of that digit.
+__device__ __forceinline__ void clear_counts(SelectShared& sh) { sh.hist[threadIdx.x] = sh.hist[threadIdx.x + kSelectThreads] = 0; }
 template <int EACH>
 __device__ __forceinline__ void count_digits(SelectShared& sh, const Entries<EACH>& t, uint32_t prefix, int q) {
-  sh.hist[threadIdx.x] = sh.hist[threadIdx.x + kSelectThreads] = 0;
-  __syncthreads();
 #pragma unroll
   for (int e = 0; e < EACH; ++e)
     if ((t.open >> e & 1) && digits_above(t.u[e], q) == prefix) atomicAdd(&sh.hist[digit_of(t.u[e], q)], 1u);
@@ -242,14 +299,14 @@ __device__ __forceinline__ uint32_t find_digit(SelectShared& sh, const int (&cnt
 // of those equal to it the first `need` (equal of which are in earlier chunks).  rank: entries of earlier chunks that
 // stay for another reason.
 template <int EACH>
-__device__ __forceinline__ void write_kept(SelectShared& sh, const Entries<EACH>& t, int first, int n, int m, uint32_t least, int need, int rank,
-                                           int equal, int* kept, float* y) {
+__device__ __forceinline__ void write_kept(SelectShared& sh, const Entries<EACH>& t, int first, int m, uint32_t least, int need, int rank, int equal,
+                                           int* kept, float* y) {
   const int i0 = first + EACH * int(threadIdx.x);
   uint32_t stays = 0, equals = 0;
 #pragma unroll
   for (int e = 0; e < EACH; ++e) {
     const bool open = t.open >> e & 1;
-    stays |= uint32_t(i0 + e < n && (!open || t.u[e] > least)) << e;
+    stays |= uint32_t((t.live >> e & 1) && (!open || t.u[e] > least)) << e;
     equals |= uint32_t(open && t.u[e] == least) << e;
   }
   // (both halves of the sums stay below 2^16: a chunk has at most 2^14 entries)
@@ -284,9 +341,28 @@ __global__ __launch_bounds__(kSelectThreads) void paged_select_kernel(const Evic
   const int rows = a.c.B * a.c.Hkv, chunk = blockIdx.x / rows, row = blockIdx.x % rows, hkv = row % a.c.Hkv, b = row / a.c.Hkv;
   const int tid = threadIdx.x, first = chunk * kChunk;
   const bool last = a.chunks == 1 || stage == kDigits;
+  const bool begin = a.chunks == 1 || stage == 0;
+  const int* table = a.c.table + int64_t(b) * a.c.table_stride;
+  // what this workgroup hands on to the next launch: its prefix, need and prior, and `live`
+  int* state = a.state + (int64_t(row) * a.chunks + chunk) * kSelectState;
+  // (loads return in order: what the first steps need is asked for before the weights)
+  const int seen = begin && tid < a.c.table_width ? table[tid] : 0;
+  Live live{};
+  if (!begin) live = Live{state[3], state[4], state[5], state[6], state[7]};
+  const int n = seq_len(a.c, b);
   Entries<EACH> t;
   read_entries(t, a.sums + int64_t(b) * a.ssum[0] + int64_t(hkv) * a.ssum[1], first, a.sums_width);
-  const int n = seq_len(a.c, b), m = imin(n, a.keep);
+  clear_counts(sh);  // (a barrier, of count_live or of find_digit, is before their use)
+  if (begin) live = count_live(sh, a.c, table, seen, n, imin(a.S, n), imax(n - a.R, 0), imin(first, n));
+  if (!last && stage == 0 && tid == 0) {
+    state[3] = live.gaps;
+    state[4] = live.all;
+    state[5] = live.lo;
+    state[6] = live.hi;
+    state[7] = live.first;
+  }
+  const bool evicts = live.all > a.keep;
+  const int m = evicts ? a.keep : live.all;
   float* y = a.new_sums + int64_t(b) * a.snew[0] + int64_t(hkv) * a.snew[1];
   if (last) {
     if (hkv == 0 && chunk == 0 && tid == 0) a.new_lens[b] = m;
@@ -294,14 +370,13 @@ __global__ __launch_bounds__(kSelectThreads) void paged_select_kernel(const Evic
     for (int i = imax(m, first) + tid; i < end; i += kSelectThreads) y[i] = 0.f;
   }
   // (entries to choose from: all but the first S and the last R, none where nothing is evicted or all stay by their place)
-  const int choose = n > a.keep ? a.keep - a.S - a.R : 0;
+  const int choose = evicts ? a.keep - live.lo - (live.all - live.hi) : 0;
   if (first >= n || (choose == 0 && !last)) return;
-  const int lo = n > a.keep ? a.S : 0, hi = n > a.keep ? n - a.R : 0;
+  const int lo = evicts ? a.S : 0, hi = evicts ? n - a.R : 0;
   uint32_t prefix = choose > 0 ? 0u : 0xffffffffu;  // (nothing to choose: no number is above, and none equal is needed)
   int need = choose, prior = 0, equal = 0;
   if (choose > 0 && a.chunks > 1 && stage > 0) {
     const int chunks = (n + kChunk - 1) / kChunk;
-    int* state = a.state + (int64_t(row) * a.chunks + chunk) * 3;  // this workgroup's prefix, need and prior
     if (stage > 1) {
       prefix = uint32_t(state[0]);
       need = state[1];
@@ -326,7 +401,7 @@ __global__ __launch_bounds__(kSelectThreads) void paged_select_kernel(const Evic
       state[2] = prior;
     }
   }
-  order_entries(t, first, lo, hi);
+  order_entries(t, a.c, table, live.gaps, first, n, lo, hi);
   if (!last) {  // counts: [digit][chunk][2047 - value]
     count_digits(sh, t, prefix, stage);
     reinterpret_cast<uint32_t*>(a.counts + ((int64_t(row) * kDigits + stage) * a.chunks + chunk) * kBins)[tid] =
@@ -335,13 +410,18 @@ __global__ __launch_bounds__(kSelectThreads) void paged_select_kernel(const Evic
   }
   if (choose > 0 && a.chunks == 1) {
     for (int q = 0; q < kDigits; ++q) {
+      if (q) {
+        clear_counts(sh);
+        __syncthreads();
+      }
       count_digits(sh, t, prefix, q);
       const int cnt[2] = {int(sh.hist[kBins - 1 - 2 * tid]), int(sh.hist[kBins - 2 - 2 * tid])}, old[2] = {0, 0};
       prefix = with_digit(prefix, find_digit<false>(sh, cnt, old, need, prior, equal), q);
     }
   }
-  const int fixed = n > a.keep ? imin(first, lo) + imax(0, first - hi) : first;  // entries of earlier chunks that stay by their place
-  write_kept(sh, t, first, n, m, prefix, need, fixed + prior, equal, a.kept + int64_t(row) * a.keep, y);
+  // entries of earlier chunks that stay by their place
+  const int fixed = evicts ? imin(live.first, live.lo) + imax(0, live.first - live.hi) : live.first;
+  write_kept(sh, t, first, m, prefix, need, fixed + prior, equal, a.kept + int64_t(row) * a.keep, y);
 }
 
 // A workgroup has kThreads / pieces entries a round.  Rounds of 1 / 2 / 4 / 8: 15.7 / 13.6 / 15.6 / 18.4 us for 8 sequences, 17.2 / 16.6 /
@@ -356,7 +436,7 @@ template <int PIECES, bool ACROSS>
 __global__ __launch_bounds__(kThreads) void paged_gather_kernel(const EvictArgs a, int chunks) {
   constexpr int ROWS = kThreads / PIECES;
   const int chunk = blockIdx.x % chunks, s = blockIdx.x / chunks, b = ACROSS ? s : s / a.c.Hkv;
-  const int n = seq_len(a.c, b), m = imin(n, a.keep);
+  const int n = seq_len(a.c, b), m = a.new_lens[b];
   const int* from = a.c.table + int64_t(b) * a.c.table_stride;
   const int* to = a.new_table + int64_t(b) * a.new_table_stride;
   const int piece = threadIdx.x % PIECES;
@@ -364,7 +444,7 @@ __global__ __launch_bounds__(kThreads) void paged_gather_kernel(const EvictArgs 
   for (int x = 0; x < kGatherRounds; ++x) {
     const int e = (chunk * kGatherRounds + x) * ROWS + int(threadIdx.x) / PIECES;
     const int r = ACROSS ? e / a.c.Hkv : e, hkv = ACROSS ? e % a.c.Hkv : s % a.c.Hkv;
-    if (r >= m) continue;
+    if (r >= m || r >= a.keep) continue;
     const int i = a.kept[(int64_t(b) * a.c.Hkv + hkv) * a.keep + r];
     if (i < 0 || i >= n) continue;  // (never, unless lens or weights change under the running call)
     const int pi = page_of(a.c.div, i), slot = i - pi * a.c.page_size, qi = page_of(a.c.div, r), new_slot = r - qi * a.c.page_size;

@@ -64,7 +64,8 @@ def paged_evict(k_pages, v_pages, block_table, lens, weight_sums, keep: int, new
     the last `recent` entries stay, and of the others those with the largest weight_sums [B, Hkv, tokens] (the lower
     position first among equals; a NaN counts as the largest).  The entries go, in order, to the pages of
     new_table (int32 [B, width]): pages that the call does not read, so that a prefix shared with other
-    sequences stays whole; sequences of at most `keep` tokens are copied.  Returns (new lens [B], new weight sums, shaped
+    sequences stays whole; sequences of at most `keep` tokens are copied.  Entries on no page of block_table are none of
+    the sequence's: they neither count nor stay.  Returns (new lens [B], new weight sums, shaped
     as weight_sums, zero behind the kept entries), to be used with new_table from then on.  An entry's place says
     nothing about its token's position any more: call paged_attention with window_size None and sink_size 0."""
     return _ops.paged_evict(k_pages, v_pages, block_table, lens, weight_sums, int(keep), new_table, int(sink_size), int(recent))

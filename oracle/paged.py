@@ -82,12 +82,13 @@ def attention(q, k_pages, v_pages, table, lens, window=None, sink=0, sinks=None,
     return o, mag, sums
 
 
-def kept(w, n, keep, sink, recent):
-    """Positions that stay of one (sequence, KV head) with weights w."""
-    if n <= keep:
-        return list(range(n))
-    held = [i for i in range(n) if i < sink or i >= n - recent]
-    rest = [i for i in range(n) if sink <= i < n - recent]
+def kept(w, n, keep, sink, recent, live=None):
+    """Positions that stay of one (sequence, KV head) with weights w; live: those on a page (None: all of n)."""
+    live = list(range(n)) if live is None else live
+    if len(live) <= keep:
+        return live
+    held = [i for i in live if i < sink or i >= n - recent]
+    rest = [i for i in live if sink <= i < n - recent]
     key = [math.inf if math.isnan(x) else x for x in w[:n].tolist()]
     first = [0 if math.isnan(x) else 1 for x in w[:n].tolist()]  # (a NaN above every number)
     rest.sort(key=lambda i: (first[i], -key[i], i))
@@ -95,18 +96,19 @@ def kept(w, n, keep, sink, recent):
 
 
 def evict(k_pages, v_pages, table, lens, sums, keep, new_table, sink=0, recent=0):
-    """New contents of (k_pages, v_pages), new lens, new sums."""
+    """New contents of (k_pages, v_pages), new lens, new sums.  Positions on no page are none of the sequence's."""
     kp, vp = k_pages.clone(), v_pages.clone()
     P, H, S, _ = kp.shape
     new, left = torch.zeros_like(sums), []
     for b in range(table.shape[0]):
         n = max(0, min(int(lens[b]), table.shape[1] * S))
-        left.append(min(n, keep))
+        live = [i for i in range(n) if entry(table, b, i, S, P) is not None]
+        left.append(min(len(live), keep))
         for h in range(H):
-            for r, i in enumerate(kept(sums[b, h], n, keep, sink, recent)):
+            for r, i in enumerate(kept(sums[b, h], n, keep, sink, recent, live)):
                 new[b, h, r] = sums[b, h, i]
                 src, dst = entry(table, b, i, S, P), entry(new_table, b, r, S, P)
-                if src is not None and dst is not None:
+                if dst is not None:
                     kp[dst[0], h, dst[1]] = k_pages[src[0], h, src[1]]
                     vp[dst[0], h, dst[1]] = v_pages[src[0], h, src[1]]
     return kp, vp, torch.tensor(left, dtype=torch.int32), new
