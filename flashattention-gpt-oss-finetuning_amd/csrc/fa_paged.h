@@ -61,8 +61,8 @@ struct PagedAttnArgs {
   // workspace
   int* starts;            // split calls: [B] the sequences' first units, and the units of a part
   float* part_o;          // [Hkv row_tiles][parts][2][16][D]
-  float* part_ml;         // [Hkv row_tiles][parts][2][2][16]: maximum (log2 domain), sum
-  float* norm;            // with sums: [B][Hq] maximum (log2 domain) and 1 / sum, of the sequences that one workgroup took whole
+  float* part_ml;         // [Hkv row_tiles][parts][2][2][16]: what weights were taken against (log2 domain), their sum
+  float* norm;            // with sums: [B][Hq] the same and 1 / sum, of the sequences that one workgroup took whole
   float* logits;          // with sums: [Hkv][B][max_units][G][kPagedUnit] (log2 domain)
 };
 

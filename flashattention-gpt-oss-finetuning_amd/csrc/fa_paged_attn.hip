@@ -13,8 +13,10 @@
 //     operand is eight V entries of keys 8j..8j+7, of which the lane loads D / 16 neighbouring dims each and pairs
 //     two keys' halves (one v_perm per register).  Its C rows are the lane's own head again, so
 //     maximum, sum and rescaling need no exchange.
-// The running maximum is raised only where a key's weight against it would exceed 2^8 (which 16 bits and float32 hold as
-// well as 1), after the first tiles hardly ever; only then do lanes exchange maxima.
+// Weights are taken against a running reference, which is raised to the maximum only where a weight would exceed 2^8 (which 16
+// bits and float32 hold as well as 1), after the first tiles hardly ever; only then do lanes exchange maxima.  float16
+// has no numbers below 2^-24: there the reference lies 2^7 below the maximum, so that weights reach 2^15 and what a key
+// can lose is 2^-32 of the largest weight, not 2^-25 (which 100000 keys of a long cache would add up to 2^-8).
 // K is loaded with neighbouring lanes on neighbouring 16-byte pieces and turned into fragments in the wave's own LDS: loaded
 // as fragments (16 rows an instruction) 876 MB took 190 us, so 166.
 // P goes into the 16-bit product as the sum of two 16-bit parts (P rounded, and what that left), so o carries its own
@@ -103,15 +105,18 @@ __device__ __forceinline__ void find_unit(const PagedAttnArgs& a, Units x, int u
   start = 0;
 }
 
-// Element types.  EB, CB: bytes of a query and of a cache element.
+// Element types.  EB, CB: bytes of a query and of a cache element.  kBelow: log2 of how far a new reference lies below the maximum.
 struct PBF16 : BF16 {
   static constexpr int EB = 2, CB = 2;
+  static constexpr float kBelow = 0.f;
 };
 struct PF16 : F16 {
   static constexpr int EB = 2, CB = 2;
+  static constexpr float kBelow = 7.f;
 };
 struct PBF16Q8 : BF16 {
   static constexpr int EB = 2, CB = 1;
+  static constexpr float kBelow = 0.f;
   static __device__ __forceinline__ uint32_t widen(uint32_t x, bool hi) {
     return hi ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, 1.0f, true))
               : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, 1.0f, false));
@@ -119,6 +124,7 @@ struct PBF16Q8 : BF16 {
 };
 struct PF16Q8 : F16 {
   static constexpr int EB = 2, CB = 1;
+  static constexpr float kBelow = 7.f;
   static __device__ __forceinline__ uint32_t widen(uint32_t x, bool hi) {
     return hi ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, 1.0f, true))
               : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, 1.0f, false));
@@ -126,6 +132,7 @@ struct PF16Q8 : F16 {
 };
 struct PF32 {
   static constexpr int EB = 4, CB = 4;
+  static constexpr float kBelow = 0.f;
 };
 
 __device__ __forceinline__ float quarters_max(float x) {
@@ -169,7 +176,7 @@ struct Wave {
   static constexpr int NQ = F ? D / 16 : (D >= 32 ? D / 32 : 1);
   u32x4 q[RT][NQ];
   f32x4 acc[RT][NC];
-  float m[RT], mref[RT], l[RT];  // running maximum (log2 domain), the same with 0 for none, this lane's sum
+  float m[RT], mref[RT], l[RT];  // running reference (log2 domain), the same with 0 for none, this lane's sum against it
 
   // Q as the B operand: head r of the tile, dims in the order in which the K pieces hold them.
   __device__ __forceinline__ void load_q(int x, const uint8_t* q_row, bool have) {
@@ -326,8 +333,8 @@ struct Wave {
       float mx = s[0];
 #pragma unroll
       for (int e = 1; e < 8; ++e) mx = fmaxf(mx, s[e]);
-      if (wave_any(mx > m[x] + 8.f)) {
-        const float up = fmaxf(m[x], quarters_max(mx));
+      if (wave_any(mx > m[x] + (8.f + E::kBelow))) {
+        const float up = fmaxf(m[x], quarters_max(mx) - E::kBelow);
         const float scale = m[x] == kNegInf ? 0.f : fast_exp2(m[x] - up);
         l[x] *= scale;
 #pragma unroll
