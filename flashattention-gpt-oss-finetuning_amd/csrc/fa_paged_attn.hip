@@ -16,11 +16,13 @@
 // Weights are taken against a running reference, which is raised to the maximum only where a weight would exceed 2^8 (which 16
 // bits and float32 hold as well as 1), after the first tiles hardly ever; only then do lanes exchange maxima.  float16
 // has no numbers below 2^-24: there the reference lies 2^7 below the maximum, so that weights reach 2^15 and what a key
-// can lose is 2^-32 of the largest weight, not 2^-25 (which 100000 keys of a long cache would add up to 2^-8).
+// can lose is 2^-32 of the largest weight of its wave's run, not 2^-25.
 // K is loaded with neighbouring lanes on neighbouring 16-byte pieces and turned into fragments in the wave's own LDS: loaded
 // as fragments (16 rows an instruction) 876 MB took 190 us, so 166.
 // P goes into the 16-bit product as the sum of two 16-bit parts (P rounded, and what that left), so o carries its own
-// rounding only; the second product costs matrix time that the loads leave idle.  float32 uses v_mfma_f32_16x16x4.
+// rounding only; the second product costs matrix time that the loads leave idle.  It sees infinite values as the largest finite
+// ones, for what the rounding left may be 0 or have the other sign: the first product decides (two operations a register of V:
+// 32 ragged sequences 52.7 -> 53.4 us).  float32 uses v_mfma_f32_16x16x4.
 //
 // Keys are addressed through a wave's own LDS table of 64-bit offsets, 64 keys at a time: key -> page -> offset is worked
 // out once a key, ahead of its use.  Keys on no page (an entry outside [0, pages)) and those past the end are marked in a
@@ -109,10 +111,12 @@ __device__ __forceinline__ void find_unit(const PagedAttnArgs& a, Units x, int u
 struct PBF16 : BF16 {
   static constexpr int EB = 2, CB = 2;
   static constexpr float kBelow = 0.f;
+  static constexpr uint16_t kLargest = 0x7f7f;
 };
 struct PF16 : F16 {
   static constexpr int EB = 2, CB = 2;
   static constexpr float kBelow = 7.f;
+  static constexpr uint16_t kLargest = 0x7bff;
 };
 struct PBF16Q8 : BF16 {
   static constexpr int EB = 2, CB = 1;
@@ -148,6 +152,16 @@ template <bool ONCE, typename T>
 __device__ __forceinline__ T fetch(const T* p) {
   if constexpr (ONCE) return __builtin_nontemporal_load(p);
   else return *p;
+}
+
+// Eight 16-bit numbers, the infinite ones (and NaN) as the largest finite ones of their sign: as integers, those of both signs are the
+// ones above it, unsigned for the negative ones and signed for the others.
+template <typename E>
+__device__ __forceinline__ u32x4 finite8(u32x4 x) {
+  typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
+  typedef int16_t i16x8 __attribute__((ext_vector_type(8)));
+  const u16x8 neg = __builtin_elementwise_min(__builtin_bit_cast(u16x8, x), u16x8(uint16_t(E::kLargest | 0x8000)));
+  return __builtin_bit_cast(u32x4, __builtin_elementwise_min(__builtin_bit_cast(i16x8, neg), i16x8(int16_t(E::kLargest))));
 }
 
 // One wave's tile of 32 keys in registers.
@@ -381,10 +395,11 @@ struct Wave {
       for (int c = 0; c < NC; ++c) {
         const u32x4 f = v_frag(w, c);
 #pragma unroll
-        for (int x = 0; x < RT; ++x) {
-          acc[x][c] = E::mfma16(f, hi[x], acc[x][c]);
-          acc[x][c] = E::mfma16(f, lo[x], acc[x][c]);
-        }
+        for (int x = 0; x < RT; ++x) acc[x][c] = E::mfma16(f, hi[x], acc[x][c]);
+        u32x4 g = f;
+        if constexpr (E::CB == 2) g = finite8<E>(f);  // (e4m3 has no infinities)
+#pragma unroll
+        for (int x = 0; x < RT; ++x) acc[x][c] = E::mfma16(g, lo[x], acc[x][c]);
       }
     }
   }

@@ -295,7 +295,8 @@ int fa_paged_append(const fa_paged_cache* c, const void* k, const void* v, const
 
 /* Attention of the last token of every sequence over its cache: query head h of sequence b sees key k < lens[b] where
  * lens[b] - 1 - k < window or k < sink.  Learned sinks (float32 [Hq]) are optional (NULL), as in fa_fwd_sinks.  A sequence
- * that sees no key gets o = 0.  With weight_sums (float32 [batch, Hkv, at least min(max_len, table tokens)], NULL: none) the
+ * that sees no key gets o = 0.  An infinite value that it sees makes o infinite (NaN with one of the other sign, and where its weight
+ * underflows: 2^-32 of the largest for fp16, 2^-126 for the other types).  With weight_sums (float32 [batch, Hkv, at least min(max_len, table tokens)], NULL: none) the
  * softmax weights are accumulated: weight_sums[b, h, k] += sum over the query heads of KV head h of P[k], in a fixed
  * order.  max_len bounds lens (they are cut off there); it and the table's width size the grid and the workspace, of
  * which at least fa_paged_workspace_bytes() are needed, 256-byte aligned. */
