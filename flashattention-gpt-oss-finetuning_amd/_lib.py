@@ -57,6 +57,7 @@ EXPORTS = (
     "fa_paged_attention",
     "fa_paged_evict_workspace_bytes",
     "fa_paged_evict",
+    "fa_check_paged_evict",
     "fa_bwd_workspace_bytes",
     "fa_bwd_full_workspace_bytes",
     "fa_check_fwd",
@@ -246,6 +247,7 @@ def lib() -> ctypes.CDLL:
             L.fa_paged_evict_workspace_bytes.argtypes = [ctypes.c_int32] * 4
             L.fa_paged_evict_workspace_bytes.restype = ctypes.c_size_t
             L.fa_paged_evict.argtypes = [ctypes.POINTER(PagedEvictParams), ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
+            L.fa_check_paged_evict.argtypes = [ctypes.POINTER(PagedEvictParams)]
             L.fa_check_fwd.argtypes = [ctypes.POINTER(FwdParams)]
             L.fa_check_fwd.restype = ctypes.c_int
             L.fa_check_bwd.argtypes = [ctypes.POINTER(BwdParams)]

@@ -661,6 +661,8 @@ def paged_evict(k_pages, v_pages, block_table, lens, weight_sums, keep: int, new
     p.new_table_width = _fits_i32(new_table.shape[1], "the new_table's width")
     p.new_lens = new_lens.data_ptr()
     p.keep, p.sink, p.recent = _fits_i32(keep, "keep"), _fits_i32(sink, "sink_size"), _fits_i32(recent, "recent")
+    # (before room is made for `keep` entries a head)
+    _lib.raise_for_status(_lib.lib().fa_check_paged_evict(ctypes.byref(p)), "fa_paged_evict")
     tokens = _i32(p.cache.table_width * p.cache.page_size)
     nbytes = int(_lib.lib().fa_paged_evict_workspace_bytes(B, Hkv, p.keep, tokens))
     ws = torch.empty((max(nbytes, 256),), dtype=torch.uint8, device=lens.device)

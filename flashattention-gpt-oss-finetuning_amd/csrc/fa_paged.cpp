@@ -190,6 +190,31 @@ EvictRoom evict_room(int64_t heads, int32_t keep, int64_t tokens) {
   return r;
 }
 
+// Everything of an eviction but its workspace.
+int check_evict(const fa_paged_evict_params* p, EvictRoom* room) {
+  if (!p) return FA_ERR_NULL;
+  const fa_paged_cache& c = p->cache;
+  const int rc = check_cache(c);
+  if (rc != FA_OK) return rc;
+  if (!p->sums || !p->new_sums || !p->new_table || !p->new_lens) return FA_ERR_NULL;
+  const int64_t tokens = int64_t(c.table_width) * c.page_size;
+  if (p->keep < 1 || p->sink < 0 || p->recent < 0 || int64_t(p->sink) + p->recent > p->keep || p->sums_width < tokens ||
+      p->new_table_width < 1 || int64_t(p->new_table_width) * c.page_size < p->keep)
+    return FA_ERR_PAGES;
+  const int64_t heads = int64_t(c.batch) * c.heads_kv;
+  if (p->keep >= fa::kPagedMaxTokens || !fa::grid_fits(heads)) return FA_ERR_OVERFLOW;
+  if (!aligned(p->sums, 4) || !aligned(p->new_sums, 4) || !aligned(p->new_table, 4) || !aligned(p->new_lens, 4) ||
+      p->new_table_stride < 0)
+    return FA_ERR_ALIGN;
+  for (int i = 0; i < 2; ++i)
+    if (p->sums_stride[i] < 0 || p->new_sums_stride[i] < 0) return FA_ERR_ALIGN;
+  // workgroups of the launches: 1024 threads a chunk, and one for each kGatherPieces of kept entries
+  const int64_t chunk = fa::kGatherPieces / (c.head_dim * elem_bytes(c.dtype) / 16);
+  *room = evict_room(heads, p->keep, tokens);
+  if (!fa::grid_fits(heads * room->chunks, 1024) || !fa::grid_fits(heads * ((p->keep + chunk - 1) / chunk))) return FA_ERR_OVERFLOW;
+  return FA_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -284,30 +309,17 @@ size_t fa_paged_evict_workspace_bytes(int32_t batch, int32_t heads_kv, int32_t k
   return r.kept + r.state + r.counts;
 }
 
+int fa_check_paged_evict(const fa_paged_evict_params* p) {
+  EvictRoom room;
+  return check_evict(p, &room);
+}
+
 int fa_paged_evict(const fa_paged_evict_params* p, void* workspace, size_t workspace_bytes, void* stream) {
-  if (!p) return FA_ERR_NULL;
-  const fa_paged_cache& c = p->cache;
-  const int rc = check_cache(c);
+  EvictRoom room;
+  const int rc = check_evict(p, &room);
   if (rc != FA_OK) return rc;
-  if (!p->sums || !p->new_sums || !p->new_table || !p->new_lens) return FA_ERR_NULL;
-  const int64_t tokens = int64_t(c.table_width) * c.page_size;
-  if (p->keep < 1 || p->sink < 0 || p->recent < 0 || int64_t(p->sink) + p->recent > p->keep || p->sums_width < tokens ||
-      p->new_table_width < 1 || int64_t(p->new_table_width) * c.page_size < p->keep)
-    return FA_ERR_PAGES;
-  const int64_t heads = int64_t(c.batch) * c.heads_kv;
-  if (p->keep >= fa::kPagedMaxTokens || !fa::grid_fits(heads)) return FA_ERR_OVERFLOW;
-  if (!aligned(p->sums, 4) || !aligned(p->new_sums, 4) || !aligned(p->new_table, 4) || !aligned(p->new_lens, 4) ||
-      p->new_table_stride < 0)
-    return FA_ERR_ALIGN;
-  for (int i = 0; i < 2; ++i)
-    if (p->sums_stride[i] < 0 || p->new_sums_stride[i] < 0) return FA_ERR_ALIGN;
-  if (!workspace || !aligned(workspace, 256) || workspace_bytes < fa_paged_evict_workspace_bytes(c.batch, c.heads_kv, p->keep, int32_t(tokens)))
-    return FA_ERR_WORKSPACE;
-  const int row = c.head_dim * elem_bytes(c.dtype);
-  // workgroups of the launches: 1024 threads a chunk, and one for each kGatherPieces of kept entries
-  const int64_t chunk = fa::kGatherPieces / (row / 16);
-  const EvictRoom room = evict_room(heads, p->keep, tokens);
-  if (!fa::grid_fits(heads * room.chunks, 1024) || !fa::grid_fits(heads * ((p->keep + chunk - 1) / chunk))) return FA_ERR_OVERFLOW;
+  const fa_paged_cache& c = p->cache;
+  if (!workspace || !aligned(workspace, 256) || workspace_bytes < room.kept + room.state + room.counts) return FA_ERR_WORKSPACE;
   fa::EvictArgs a{};
   a.c = cache_args(c);
   a.sums = p->sums;
@@ -329,7 +341,7 @@ int fa_paged_evict(const fa_paged_evict_params* p, void* workspace, size_t works
   a.kept = reinterpret_cast<int*>(ws);
   a.state = reinterpret_cast<int*>(ws + room.kept);
   a.counts = reinterpret_cast<uint16_t*>(ws + room.kept + room.state);
-  return status(fa::launch_paged_evict(a, row, static_cast<hipStream_t>(stream)));
+  return status(fa::launch_paged_evict(a, c.head_dim * elem_bytes(c.dtype), static_cast<hipStream_t>(stream)));
 }
 
 }  // extern "C"

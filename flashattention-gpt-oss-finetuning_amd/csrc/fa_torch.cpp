@@ -717,6 +717,7 @@ std::vector<at::Tensor> paged_evict(const at::Tensor& k_pages, const at::Tensor&
   p.keep = to_i32(kept, "keep");
   p.sink = to_i32(sink, "sink_size");
   p.recent = to_i32(recent, "recent");
+  raise_for_status(fa_check_paged_evict(&p), "fa_paged_evict");  // (before room is made for `keep` entries a head)
   const size_t bytes = fa_paged_evict_workspace_bytes(p.cache.batch, p.cache.heads_kv, p.keep, clamp_i32(table.size(1) * k_pages.size(2)));
   at::Tensor ws = at::empty({int64_t(bytes > 256 ? bytes : 256)}, sums.options().dtype(at::kByte));
   raise_for_status(fa_paged_evict(&p, ws.data_ptr(), size_t(ws.numel()), current_stream(sums)), "fa_paged_evict");

@@ -338,6 +338,8 @@ typedef struct fa_paged_evict_params {
 } fa_paged_evict_params;
 size_t fa_paged_evict_workspace_bytes(int32_t batch, int32_t heads_kv, int32_t keep, int32_t tokens);
 int fa_paged_evict(const fa_paged_evict_params* p, void* workspace, size_t workspace_bytes, void* stream);
+/* Host-only argument check used by fa_paged_evict (no HIP call is made, no workspace needed yet). */
+int fa_check_paged_evict(const fa_paged_evict_params* p);
 
 /* Host-only argument checks used by fa_fwd / fa_bwd (no HIP call is made). */
 int fa_check_fwd(const fa_fwd_params* p);
