@@ -27,7 +27,8 @@ Answering with a model (paged.py): a paged key-value cache, one new token a sequ
     paged_append(k, v, k_pages, v_pages, block_table, lens, cu_seqlens=None, descale=(1.0, 1.0))
     paged_attention(q, k_pages, v_pages, block_table, lens, window_size=None, sink_size=0, sinks=None,
                     scale=None, descale=(1.0, 1.0), max_seqlen=None, weight_sums=None)
-    paged_evict(k_pages, v_pages, block_table, lens, weight_sums, keep, new_table, sink_size=0, recent=0)
+    paged_evict(k_pages, v_pages, block_table, lens, weight_sums, keep, new_table, sink_size=0, recent=0,
+                max_seqlen=None)
 
 The directory name is not a Python identifier; import it with
 ``importlib.import_module("flashattention-gpt-oss-finetuning_amd")`` from the repository root.

@@ -184,6 +184,7 @@ class PagedEvictParams(ctypes.Structure):
         ("keep", ctypes.c_int32),
         ("sink", ctypes.c_int32),
         ("recent", ctypes.c_int32),
+        ("max_len", ctypes.c_int32),
     ]
 
 

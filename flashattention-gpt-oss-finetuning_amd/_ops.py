@@ -634,11 +634,11 @@ def paged_attention(q, k_pages, v_pages, block_table, lens, window: int, sink: i
     return o
 
 
-def paged_evict(k_pages, v_pages, block_table, lens, weight_sums, keep: int, new_table, sink: int, recent: int):
-    """fa_paged_evict: (new lens, new weight sums)."""
+def paged_evict(k_pages, v_pages, block_table, lens, weight_sums, keep: int, new_table, sink: int, recent: int, max_len: int = 0):
+    """fa_paged_evict: (new lens, new weight sums); max_len 0: the table's tokens."""
     b = _binding()
     if b is not None:
-        return tuple(b.paged_evict(k_pages, v_pages, block_table, lens, weight_sums, keep, new_table, sink, recent))
+        return tuple(b.paged_evict(k_pages, v_pages, block_table, lens, weight_sums, keep, new_table, sink, recent, max_len))
     _refuse_traced("paged_evict")
     p = _lib.PagedEvictParams()
     p.cache, held = _paged_cache(k_pages, v_pages, block_table, lens, 1.0, 1.0)
@@ -661,9 +661,11 @@ def paged_evict(k_pages, v_pages, block_table, lens, weight_sums, keep: int, new
     p.new_table_width = _fits_i32(new_table.shape[1], "the new_table's width")
     p.new_lens = new_lens.data_ptr()
     p.keep, p.sink, p.recent = _fits_i32(keep, "keep"), _fits_i32(sink, "sink_size"), _fits_i32(recent, "recent")
+    p.max_len = _fits_i32(max_len, "max_seqlen")
     # (before room is made for `keep` entries a head)
     _lib.raise_for_status(_lib.lib().fa_check_paged_evict(ctypes.byref(p)), "fa_paged_evict")
-    tokens = _i32(p.cache.table_width * p.cache.page_size)
+    tokens = p.cache.table_width * p.cache.page_size
+    tokens = min(tokens, p.max_len) if p.max_len else tokens
     nbytes = int(_lib.lib().fa_paged_evict_workspace_bytes(B, Hkv, p.keep, tokens))
     ws = torch.empty((max(nbytes, 256),), dtype=torch.uint8, device=lens.device)
     _run_paged("fa_paged_evict", lens.device, ctypes.byref(p), ctypes.c_void_p(ws.data_ptr()), ctypes.c_size_t(ws.numel()))

@@ -190,6 +190,12 @@ EvictRoom evict_room(int64_t heads, int32_t keep, int64_t tokens) {
   return r;
 }
 
+// The tokens that a sequence can have in an eviction.
+int64_t evict_tokens(const fa_paged_evict_params* p) {
+  const int64_t table = int64_t(p->cache.table_width) * p->cache.page_size;
+  return p->max_len > 0 ? std::min<int64_t>(table, p->max_len) : table;
+}
+
 // Everything of an eviction but its workspace.
 int check_evict(const fa_paged_evict_params* p, EvictRoom* room) {
   if (!p) return FA_ERR_NULL;
@@ -197,7 +203,8 @@ int check_evict(const fa_paged_evict_params* p, EvictRoom* room) {
   const int rc = check_cache(c);
   if (rc != FA_OK) return rc;
   if (!p->sums || !p->new_sums || !p->new_table || !p->new_lens) return FA_ERR_NULL;
-  const int64_t tokens = int64_t(c.table_width) * c.page_size;
+  if (p->max_len < 0) return FA_ERR_SHAPE;
+  const int64_t tokens = evict_tokens(p);
   if (p->keep < 1 || p->sink < 0 || p->recent < 0 || int64_t(p->sink) + p->recent > p->keep || p->sums_width < tokens ||
       p->new_table_width < 1 || int64_t(p->new_table_width) * c.page_size < p->keep)
     return FA_ERR_PAGES;
@@ -322,6 +329,7 @@ int fa_paged_evict(const fa_paged_evict_params* p, void* workspace, size_t works
   if (!workspace || !aligned(workspace, 256) || workspace_bytes < room.kept + room.state + room.counts) return FA_ERR_WORKSPACE;
   fa::EvictArgs a{};
   a.c = cache_args(c);
+  a.c.max_len = int(evict_tokens(p));
   a.sums = p->sums;
   a.new_sums = p->new_sums;
   for (int i = 0; i < 2; ++i) {

@@ -681,7 +681,7 @@ at::Tensor paged_attention(const at::Tensor& q_in, const at::Tensor& k_pages, co
 // (new lens, new weight sums)
 std::vector<at::Tensor> paged_evict(const at::Tensor& k_pages, const at::Tensor& v_pages, const at::Tensor& table,
                                     const at::Tensor& lens, const at::Tensor& sums, int64_t kept, const at::Tensor& new_table_in,
-                                    int64_t sink, int64_t recent) {
+                                    int64_t sink, int64_t recent, int64_t max_len) {
   refuse_transformed({&k_pages, &v_pages, &sums}, "paged_evict");
   std::vector<at::Tensor> keep;
   fa_paged_evict_params p{};
@@ -717,8 +717,11 @@ std::vector<at::Tensor> paged_evict(const at::Tensor& k_pages, const at::Tensor&
   p.keep = to_i32(kept, "keep");
   p.sink = to_i32(sink, "sink_size");
   p.recent = to_i32(recent, "recent");
+  p.max_len = to_i32(max_len, "max_seqlen");
   raise_for_status(fa_check_paged_evict(&p), "fa_paged_evict");  // (before room is made for `keep` entries a head)
-  const size_t bytes = fa_paged_evict_workspace_bytes(p.cache.batch, p.cache.heads_kv, p.keep, clamp_i32(table.size(1) * k_pages.size(2)));
+  const int32_t tokens = clamp_i32(table.size(1) * k_pages.size(2));
+  const size_t bytes = fa_paged_evict_workspace_bytes(p.cache.batch, p.cache.heads_kv, p.keep,
+                                                      p.max_len ? std::min(tokens, p.max_len) : tokens);
   at::Tensor ws = at::empty({int64_t(bytes > 256 ? bytes : 256)}, sums.options().dtype(at::kByte));
   raise_for_status(fa_paged_evict(&p, ws.data_ptr(), size_t(ws.numel()), current_stream(sums)), "fa_paged_evict");
   changed(k_pages);
@@ -733,7 +736,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("paged_attention", &paged_attention,
         "(q, k_pages, v_pages, block_table, lens, window, sink, sinks, scale, k_descale, v_descale, max_len, weight_sums) -> o");
   m.def("paged_evict", &paged_evict,
-        "(k_pages, v_pages, block_table, lens, weight_sums, keep, new_table, sink, recent) -> (new lens, new weight sums)");
+        "(k_pages, v_pages, block_table, lens, weight_sums, keep, new_table, sink, recent, max_len) -> (new lens, new weight sums)");
   m.def("swda", &swda,
         "autograd forward of causal sliding-window + sink attention: (q, k, v, window, sink, scale) -> o or None",
         py::arg("q"), py::arg("k"), py::arg("v"), py::arg("window"), py::arg("sink"), py::arg("scale"));

@@ -59,7 +59,8 @@ def paged_attention(q, k_pages, v_pages, block_table, lens, window_size: Optiona
                                 most if max_seqlen is None else int(max_seqlen), weight_sums)
 
 
-def paged_evict(k_pages, v_pages, block_table, lens, weight_sums, keep: int, new_table, sink_size: int = 0, recent: int = 0):
+def paged_evict(k_pages, v_pages, block_table, lens, weight_sums, keep: int, new_table, sink_size: int = 0, recent: int = 0,
+                max_seqlen: Optional[int] = None):
     """Thins out every sequence of more than `keep` tokens to `keep` entries, each KV head by itself: the first sink_size and
     the last `recent` entries stay, and of the others those with the largest weight_sums [B, Hkv, tokens] (the lower
     position first among equals; a NaN counts as the largest).  The entries go, in order, to the pages of
@@ -67,5 +68,10 @@ def paged_evict(k_pages, v_pages, block_table, lens, weight_sums, keep: int, new
     sequences stays whole; sequences of at most `keep` tokens are copied.  Entries on no page of block_table are none of
     the sequence's: they neither count nor stay.  Returns (new lens [B], new weight sums, shaped
     as weight_sums, zero behind the kept entries), to be used with new_table from then on.  An entry's place says
-    nothing about its token's position any more: call paged_attention with window_size None and sink_size 0."""
-    return _ops.paged_evict(k_pages, v_pages, block_table, lens, weight_sums, int(keep), new_table, int(sink_size), int(recent))
+    nothing about its token's position any more: call paged_attention with window_size None and sink_size 0.
+
+    max_seqlen: a bound on lens, as paged_attention's; weight_sums are that wide at least."""
+    if max_seqlen is not None and max_seqlen < 1:
+        raise ValueError(f"max_seqlen must be at least 1, got {max_seqlen}")
+    return _ops.paged_evict(k_pages, v_pages, block_table, lens, weight_sums, int(keep), new_table, int(sink_size), int(recent),
+                            0 if max_seqlen is None else min(int(max_seqlen), 2 ** 31 - 1))

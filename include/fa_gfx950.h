@@ -324,7 +324,8 @@ int fa_paged_attention(const fa_paged_attention_params* p, void* workspace, size
  * shorter sequences are copied whole.  Positions on no page (see above) are none of the sequence's: they are not kept, and
  * n is the number of the others, while the first `sink` and the last `recent` are positions.  new_sums gets the kept entries'
  * sums and zeros behind them (new_sums is other memory than sums), new_lens min(n, keep).  Positions have no meaning for the window or the sinks of an attention call any more.  The
- * workspace holds at least fa_paged_evict_workspace_bytes(), whose `tokens` are the table's: table_width * page_size. */
+ * workspace holds at least fa_paged_evict_workspace_bytes(), whose `tokens` are the table's (table_width * page_size) or, if that
+ * is less, max_len; sums are that wide at least. */
 typedef struct fa_paged_evict_params {
   fa_paged_cache cache;
   const float* sums;      /* [batch, Hkv, sums_width] */
@@ -335,6 +336,7 @@ typedef struct fa_paged_evict_params {
   int64_t new_table_stride;
   int32_t* new_lens;      /* [batch] */
   int32_t sums_width, new_table_width, keep, sink, recent;
+  int32_t max_len;        /* a bound on lens, as of fa_paged_attention; 0: the table's tokens */
 } fa_paged_evict_params;
 size_t fa_paged_evict_workspace_bytes(int32_t batch, int32_t heads_kv, int32_t keep, int32_t tokens);
 int fa_paged_evict(const fa_paged_evict_params* p, void* workspace, size_t workspace_bytes, void* stream);

@@ -9,6 +9,8 @@ from test_paged_cpu import CACHE_CASES, _cache, _code, _evict, _lib
 @pytest.mark.parametrize("over,code", [
     (dict(), None), (dict(keep=1 << 28), "PAGES"), (dict(keep=0), "PAGES"), (dict(new_table_width=1 << 28, keep=1 << 30), "OVERFLOW"),
     (dict(sums=None), "NULL"), (dict(new_table_stride=-1), "ALIGN"), (dict(sums_width=159), "PAGES"),
+    (dict(sums_width=159, max_len=159), None), (dict(sums_width=159, max_len=160), "PAGES"), (dict(max_len=1 << 30), None),
+    (dict(max_len=-1), "SHAPE"),
 ], ids=lambda x: str(x))
 def test_check(over, code):
     assert _lib.lib().fa_check_paged_evict(ctypes.byref(_evict(**over))) == (0 if code is None else _code(code))
