@@ -16,7 +16,8 @@ GPU, so a step can be captured into a HIP graph.  Entries of block_table that ar
 masked when read and left out when written; a sequence with lens 0 is idle.
 
 Pages are bfloat16, float16 or float32, as the call's other tensors, or float8_e4m3fn under bfloat16 or float16
-tensors (D 64 or 128): a code stands for descale[0] (keys) or descale[1] (values) times its value.  Forward only, no autograd.
+tensors (D 64 or 128): a code stands for descale[0] (keys) or descale[1] (values) times its value.  Forward only: what
+paged_attention returns for inputs that require a gradient raises in the backward pass, and what is in the pages has none.
 Compute is in csrc/fa_paged_attn.hip and csrc/fa_paged_cache.hip; there is no CPU implementation.
 """
 from __future__ import annotations
@@ -27,6 +28,19 @@ from typing import Optional
 import torch
 
 from . import _ops
+
+
+class _NoBackward(torch.autograd.Function):
+    """o as it is, but with an error in place of a silently missing gradient."""
+
+    @staticmethod
+    def forward(ctx, o, *inputs):
+        return o
+
+    @staticmethod
+    def backward(ctx, do):
+        raise NotImplementedError("paged_attention has no backward pass; train with flash_swda_with_sink and its kin, and "
+                                  "answer under torch.no_grad()")
 
 
 def paged_append(k, v, k_pages, v_pages, block_table, lens, cu_seqlens: Optional[torch.Tensor] = None,
@@ -54,9 +68,14 @@ def paged_attention(q, k_pages, v_pages, block_table, lens, window_size: Optiona
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1])
     most = 2 ** 31 - 1
-    return _ops.paged_attention(q, k_pages, v_pages, block_table, lens, most if window_size is None else int(window_size),
-                                int(sink_size), sinks, float(scale), float(descale[0]), float(descale[1]),
-                                most if max_seqlen is None else int(max_seqlen), weight_sums)
+    o = _ops.paged_attention(q, k_pages, v_pages, block_table, lens, most if window_size is None else int(window_size),
+                             int(sink_size), sinks, float(scale), float(descale[0]), float(descale[1]),
+                             most if max_seqlen is None else int(max_seqlen), weight_sums)
+    if torch.is_grad_enabled():
+        inputs = [t for t in (q, k_pages, v_pages, sinks) if t is not None and t.requires_grad]
+        if inputs:
+            return _NoBackward.apply(o, *inputs)
+    return o
 
 
 def paged_evict(k_pages, v_pages, block_table, lens, weight_sums, keep: int, new_table, sink_size: int = 0, recent: int = 0,
