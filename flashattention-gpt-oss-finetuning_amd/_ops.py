@@ -479,8 +479,9 @@ def _fits_i32(x: int, name: str) -> int:
     return x
 
 
-def _refuse_traced(what: str) -> None:
-    if torch.jit.is_tracing() or torch.compiler.is_compiling():
+def _refuse_traced(what: str, *tensors) -> None:
+    if (torch.jit.is_tracing() or torch.compiler.is_compiling() or torch._C._functorch.peek_interpreter_stack() is not None
+            or any(t is not None and torch.autograd.forward_ad.unpack_dual(t).tangent is not None for t in tensors)):
         raise RuntimeError(f"{what} works on tensors in place: it cannot be traced or transformed")
 
 
@@ -578,7 +579,7 @@ def paged_append(k, v, k_pages, v_pages, block_table, lens, cu, k_descale: float
     b = _binding()
     if b is not None:
         return b.paged_append(k, v, k_pages, v_pages, block_table, lens, cu, k_descale, v_descale)
-    _refuse_traced("paged_append")
+    _refuse_traced("paged_append", k, v, k_pages, v_pages)
     c, held = _paged_cache(k_pages, v_pages, block_table, lens, k_descale, v_descale)
     _distinct(k_pages=k_pages, v_pages=v_pages)
     k, v = _paged_input(k, k_pages, "k"), _paged_input(v, k_pages, "v")
@@ -602,7 +603,7 @@ def paged_attention(q, k_pages, v_pages, block_table, lens, window: int, sink: i
     if b is not None:
         return b.paged_attention(q, k_pages, v_pages, block_table, lens, window, sink, sinks, scale, k_descale, v_descale, max_len,
                                  weight_sums)
-    _refuse_traced("paged_attention")
+    _refuse_traced("paged_attention", q, k_pages, v_pages, sinks, weight_sums)
     p = _lib.PagedAttentionParams()
     p.cache, held = _paged_cache(k_pages, v_pages, block_table, lens, k_descale, v_descale)
     q = _paged_input(q, k_pages, "q")
@@ -639,7 +640,7 @@ def paged_evict(k_pages, v_pages, block_table, lens, weight_sums, keep: int, new
     b = _binding()
     if b is not None:
         return tuple(b.paged_evict(k_pages, v_pages, block_table, lens, weight_sums, keep, new_table, sink, recent, max_len))
-    _refuse_traced("paged_evict")
+    _refuse_traced("paged_evict", k_pages, v_pages, weight_sums)
     p = _lib.PagedEvictParams()
     p.cache, held = _paged_cache(k_pages, v_pages, block_table, lens, 1.0, 1.0)
     _distinct(k_pages=k_pages, v_pages=v_pages)

@@ -635,7 +635,8 @@ at::Tensor paged_attention(const at::Tensor& q_in, const at::Tensor& k_pages, co
                            const at::Tensor& table, const at::Tensor& lens, int64_t window, int64_t sink,
                            const c10::optional<at::Tensor>& sinks_in, double scale, double k_descale, double v_descale,
                            int64_t max_len, const c10::optional<at::Tensor>& sums) {
-  refuse_transformed({&q_in, &k_pages, &v_pages}, "paged_attention");
+  refuse_transformed({&q_in, &k_pages, &v_pages, sinks_in.has_value() ? &*sinks_in : &q_in, sums.has_value() ? &*sums : &q_in},
+                     "paged_attention");
   std::vector<at::Tensor> keep;
   fa_paged_attention_params p{};
   p.cache = paged_cache(k_pages, v_pages, table, lens, k_descale, v_descale, keep);
