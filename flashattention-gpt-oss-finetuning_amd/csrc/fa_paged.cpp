@@ -90,9 +90,15 @@ constexpr int kSingleWgs = 1024, kSingleUnits = 2;
 // does (1 sequence of 2048 tokens: 10.3 us with at least two units each, 9.8 with one).
 constexpr int kPartsPerCu = 2, kPartsNarrow = 3, kLeastUnits = 1;
 // Where a page has its slots before its heads, the workgroups of a part's KV heads read neighbouring pieces of the same rows, and
-// twice as many and shorter runs keep them closer together: 876 MB 152 us with 2 a compute unit, 145 with 4; but 261 MB 52.7
-// and 52.6, 71 MB 17.8 and 20.3.  So the second half of the parts is used above kManyBytes of K and V.
+// twice as many and shorter runs keep them closer together, once the call is large.  With 2 / 4 a compute unit (bf16, 8 heads of
+// D = 64): 261 MB 49 / 49 us, 342 MB 65.6 / 65.0, 420 MB 79.6 / 77.2, 502 MB 95 / 92, 876 MB 158 / 150; the second launch takes 0.3 more.
+// So the second half of the parts is used above kManyBytes of K and V, and where a slot's row has kManyRow bytes at least, in
+// entries of kManyEntry at most (about 700 MB): 16 heads of D = 64 281 / 236, of D = 32 180 / 163, 32 of D = 16 286 / 272; e4m3 16 heads of D = 64
+// 181 / 163, 8 of D = 128 136 / 129; float32 8 heads of D = 32 141 / 130.  Shorter rows: 4 heads of D = 64 135 / 138, 8 of D = 32 173 / 190, 16 of
+// D = 16 309 / 341, 2 of D = 32 229 / 261; e4m3 8 heads of D = 64 168 / 175.  Longer entries, of which a compute unit has fewer workgroups at a
+// time: D = 128, 4 heads 92 / 99 (502 MB), 8 heads 244 / 247; float32 4 heads of D = 128 245 / 264, of D = 64 130 / 127.
 constexpr int64_t kManyBytes = int64_t(384) << 20;
+constexpr int kManyRow = 1024, kManyEntry = 128;
 // Loads of a call that reads more than this are marked as read once, so that they do not run through the 256 MB last-level
 // cache: 537 MB take 84 us so and 103 otherwise, 261 MB 49 and 54.  Below, the next step finds the keys there: three caches of 71 MB
 // in turn take 17.4 us each, 19.3 with marked loads.
@@ -145,7 +151,8 @@ int plan(const fa_paged_attention_params* p, Plan* r) {
     r->parts = int((std::min(want, (units + kLeastUnits - 1) / kLeastUnits) + 7) / 8 * 8);
     r->few = r->parts;
     r->many_units = int(std::min<int64_t>(kManyBytes / unit_bytes(c), INT32_MAX));
-    if (c.k_stride[1] < c.k_stride[2] && units > r->many_units) r->parts *= 2;
+    const int64_t entry = int64_t(c.head_dim) * elem_bytes(c.dtype);
+    if (c.k_stride[1] < c.k_stride[2] && entry <= kManyEntry && entry * c.heads_kv >= kManyRow && units > r->many_units) r->parts *= 2;
     if (!fa::grid_fits(streams * r->parts)) return FA_ERR_OVERFLOW;
   }
   const size_t slots = size_t(c.heads_kv) * r->row_tiles * r->parts * 2;

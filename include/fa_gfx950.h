@@ -323,7 +323,7 @@ int fa_paged_attention(const fa_paged_attention_params* p, void* workspace, size
  * positions 0, 1, ... of the pages of new_table ([batch][new_table_width]), which must not be pages that the call reads;
  * shorter sequences are copied whole.  Positions on no page (see above) are none of the sequence's: they are not kept, and
  * n is the number of the others, while the first `sink` and the last `recent` are positions.  new_sums gets the kept entries'
- * sums and zeros behind them (new_sums is other memory than sums), new_lens min(n, keep).  Positions have no meaning for the window or the sinks of an attention call any more.  The
+ * sums and zeros behind them, new_lens min(n, keep); both are other memory than sums and lens.  Positions have no meaning for the window or the sinks of an attention call any more.  The
  * workspace holds at least fa_paged_evict_workspace_bytes(), whose `tokens` are the table's (table_width * page_size) or, if that
  * is less, max_len; sums are that wide at least. */
 typedef struct fa_paged_evict_params {
