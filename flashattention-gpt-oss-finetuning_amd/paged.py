@@ -71,10 +71,9 @@ def paged_attention(q, k_pages, v_pages, block_table, lens, window_size: Optiona
     o = _ops.paged_attention(q, k_pages, v_pages, block_table, lens, most if window_size is None else int(window_size),
                              int(sink_size), sinks, float(scale), float(descale[0]), float(descale[1]),
                              most if max_seqlen is None else int(max_seqlen), weight_sums)
-    if torch.is_grad_enabled():
-        inputs = [t for t in (q, k_pages, v_pages, sinks) if t is not None and t.requires_grad]
-        if inputs:
-            return _NoBackward.apply(o, *inputs)
+    if (q.requires_grad or k_pages.requires_grad or v_pages.requires_grad or (sinks is not None and sinks.requires_grad)) \
+            and torch.is_grad_enabled():
+        return _NoBackward.apply(o, q, k_pages, v_pages, sinks)
     return o
 
 
