@@ -68,24 +68,24 @@ int status(hipError_t e) { return e == hipSuccess ? FA_OK : FA_ERR_LAUNCH; }
 // Which launch serves a call.  Sequences that see at most whole_keys() keys are taken whole, a workgroup each, in one launch; twice
 // as many where there are kManyWgs (KV head, share of its heads, sequence) triples.  Ragged batches are no reason to split here: the
 // bound is what the longest can be.  Times in us, whole / split, with 8 KV heads and D = 64 (4 and D = 128):
-//   bf16: 1 sequence of 1001 tokens 7.9 / 9.1, of 1500 9.4 / 9.1, of 2048 11.3 / 9.2; 4 of 2048 11.4 / 10.0;
-//     16 (128 workgroups) of 1500 11.7 / 16.3, of 2048 14.4 / 19.0; 64 (512 workgroups) of 2048 43.9 / 48.1, of 4096 97 / 85
-//   bf16 D = 128: 1 of 600 9.4 / 9.3, of 1000 12.6 / 9.5; 16 (64 workgroups) of 700 10.6 / 14.9, of 1000 13.4 / 16.0
+//   bf16: 1 sequence of 1001 tokens 9.1 / 9.8, of 1500 11.0 / 9.7, of 2048 12.9 / 9.8; 4 of 2048 14.2 / 12.4;
+//     16 (128 workgroups) of 1500 13.3 / 19.2, of 2048 15.9 / 21.4; 64 (512 workgroups) of 2048 51.7 / 54.1, of 4096 98 / 96
+//   bf16 D = 128: 1 of 600 10.1 / 9.9, of 1000 13.8 / 10.0; 16 (64 workgroups) of 700 12.6 / 18.8, of 1000 15.0 / 19.5
 //   e4m3: 8 (64 workgroups) of 1500 10.2 / 11.4, of 2000 12.2 / 11.4; 16 of 2000 12.9 / 14.5
 //   e4m3 D = 128: 1 of 600 8.0 / 9.2, of 1000 10.4 / 9.3; 16 (64 workgroups) of 1000 10.8 / 11.6, of 1500 14.1 / 13.2
 //   float32: 1 of 600 12.6 / 10.0 (the lines cross at about 380); 8 (64 workgroups) of 500 11.2 / 10.7; 16 of 500 11.9 / 13.3
 //   float32 D = 128: 1 of 600 21.6 / 12.4; 16 (64 workgroups) of 400 18.8 / 14.2
-//   64 heads over one: 1 of 600 8.7 / 10.8, of 1000 11.0 / 10.9; 16 of 1000 11.4 / 12.2, of 1500 14.1 / 13.7
+//   64 heads over one, bf16: 1 of 600 9.5 / 10.6, of 1000 11.9 / 10.4; 16 of 1000 12.5 / 12.6, of 1500 15.4 / 16.3
 int whole_keys(int D, int cache_bytes) {
   return cache_bytes == 4 ? (D > 64 ? 128 : 256) : D * cache_bytes > 128 ? 512 : D > 64 ? 768 : 1024;
 }
 constexpr int kManyWgs = 64;
 // Whole sequences are taken by 8 waves while there are at most as many workgroups as compute units (1 sequence of 1001
-// tokens: 9.2 us with 4 waves, 7.9 with 8; but 64 of 256: 7.4 and 9.5), and by a wave each where there are kSingleWgs of at
-// most kSingleUnits units (256 sliding-layer sequences 17.7 us with 4 waves, 14.2 with one; 1024 of them 78 and 59).
+// tokens: 10.5 us with 4 waves, 9.1 with 8; but 64 of 256: 9.8 and 12.5), and by a wave each where there are kSingleWgs of at
+// most kSingleUnits units (256 sliding-layer sequences 20.9 us with 4 waves, 15.6 with one; 1024 of them 83 and 62).
 constexpr int kSingleWgs = 1024, kSingleUnits = 2;
-// Split calls: workgroups for each compute unit.  With 1 / 2 / 3 of them 32 ragged sequences (261 MB) take 54 / 49 / 55 us, e4m3
-// D = 128 (123 MB) 30 / 27 / 33, four of up to 128K tokens (876 MB) 160 / 157 / 148.  Rows of 32 bytes make a tile as much work for a
+// Split calls: workgroups for each compute unit.  With 1 / 2 / 3 of them 32 ragged sequences (261 MB) take 53 / 49 / 55 us, e4m3
+// D = 128 (123 MB) 27 / 25 / 29, four of up to 128K tokens (876 MB) 158 / 149 / 150.  Rows of 32 bytes make a tile as much work for a
 // quarter of the bytes: 137 us with 2, 113 with 3 (537 MB).  A unit more a workgroup costs a short call more than its piece
 // does (1 sequence of 2048 tokens: 10.3 us with at least two units each, 9.8 with one).
 constexpr int kPartsPerCu = 2, kPartsNarrow = 3, kLeastUnits = 1;
@@ -100,8 +100,8 @@ constexpr int kPartsPerCu = 2, kPartsNarrow = 3, kLeastUnits = 1;
 constexpr int64_t kManyBytes = int64_t(384) << 20;
 constexpr int kManyRow = 1024, kManyEntry = 128;
 // Loads of a call that reads more than this are marked as read once, so that they do not run through the 256 MB last-level
-// cache: 537 MB take 84 us so and 103 otherwise, 261 MB 49 and 54.  Below, the next step finds the keys there: three caches of 71 MB
-// in turn take 17.4 us each, 19.3 with marked loads.
+// cache: 537 MB take 90 us so and 100 otherwise, 261 MB 49 and 54.  Below, the next step finds the keys there: three caches of 71 MB
+// in turn take 18.1 us each, 19.8 with marked loads.
 constexpr int64_t kKeepBytes = int64_t(96) << 20;
 
 // K and V bytes of a unit of keys, all KV heads.

@@ -18,7 +18,7 @@
 // has no numbers below 2^-24: there the reference lies 2^7 below the maximum, so that weights reach 2^15 and what a key
 // can lose is 2^-32 of the largest weight of its wave's run, not 2^-25.
 // K is loaded with neighbouring lanes on neighbouring 16-byte pieces and turned into fragments in the wave's own LDS: loaded
-// as fragments (16 rows an instruction) 876 MB took 190 us, so 166.
+// as fragments (16 rows an instruction) 876 MB took 190 us, so 166, all else as it was.
 // P goes into the 16-bit product as the sum of two 16-bit parts (P rounded, and what that left), so o carries its own
 // rounding only; the second product costs matrix time that the loads leave idle.  It sees infinite values as the largest finite
 // ones, for what the rounding left may be 0 or have the other sign: the first product decides (two operations a register of V:
@@ -34,11 +34,11 @@
 // sizes the host knows.  Pieces that are no whole sequence leave (maximum, sum, o) in the workspace, and
 // paged_finish_kernel joins them.
 //
-// Measured (D = 64, bf16, 8 heads a group; rocprofv3): 32 ragged sequences, 261 MB of K and V, 48 to 50 us, 5.3 TB/s; four of up to 128K
-// tokens, 876 MB, 143 us, 6.1 TB/s, with the heads before the slots in a page and with the slots first.  The
-// counters show 261 and 877 MB read: every entry once.  A plain kernel that only reads reaches 6.2 TB/s, 7.1 with loads marked as read
+// Measured (D = 64, bf16, 8 heads a group; rocprofv3): 32 ragged sequences, 261 MB of K and V, 49 to 51 us, 5.2 TB/s; four of up to 128K
+// tokens, 876 MB, 138 us, 6.3 TB/s, with the heads before the slots in a page and 147 to 150, 5.9, with the slots first.  float32: 522 MB
+// 93 us, 5.6 TB/s; with D = 128 119, 4.4.  The counters show 261 and 877 MB read: every entry once.  A plain kernel that only reads reaches 6.2 TB/s, 7.1 with loads marked as read
 // once.  Without the products and the softmax (loads only) the kernel took the same time to 5%.
-// What is left of a small call is latency: lens, table, K, four tiles, the waves' sums: one sliding-layer step 5.3 us.
+// What is left of a small call is latency: lens, table, K, four tiles, the waves' sums: one sliding-layer step 5.4 to 5.8 us.
 #include <hip/hip_runtime.h>
 
 #include "../../include/fa_gfx950.h"

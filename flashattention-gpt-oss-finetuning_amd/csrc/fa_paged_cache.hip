@@ -3,8 +3,10 @@
 //
 // paged_append_kernel.  Row i of sequence b's n new rows goes to position lens[b] - n + i.  A wave takes a row: it finds the
 // row's sequence by one ballot over cu_seqlens and the page once, then its lanes copy the 16-byte pieces of
-// every head's K and V: a prompt of 16384 rows (67 MB moved) 12.7 us, 5.3 TB/s; into e4m3 pages, D = 128 (35 MB), 10.5; a
-// decoding step of 64 rows 2.8, all latency.  Two rows a wave gained nothing (12.6, 11.2, 4.0).  e4m3 pages get the codes of clamp(x * fl32(1 / descale), -448, 448), as quantize_fp8's.
+// every head's K and V: a prompt of 16384 rows (67 MB moved) 13.0 us, 5.2 TB/s; into e4m3 pages, D = 128 (35 MB), 10.6; a
+// decoding step of 64 rows 3.1, all latency.  Two rows a wave gained nothing (12.6, 11.2, 4.0, with 12.7, 10.5, 2.8 for one).  Rows of few
+// pieces leave lanes idle: 16384 rows of one head, 8 MB with D = 64 and 4 with D = 32, take 7 us either way.  e4m3 pages get
+// the codes of clamp(x * fl32(1 / descale), -448, 448), as quantize_fp8's.
 //
 // paged_select_kernel.  Of a (sequence, KV head)'s n entries the first S and the last R stay, and of the others the
 // keep - S - R of the largest weight, the lower index first among equals (NaN counts as the largest).  Entries on no page are
@@ -12,10 +14,10 @@
 // sequence's row of the table (1 us in the first launch) says whether there are any; only then are those on pages counted.  The weights are
 // mapped to unsigned numbers of the same order; three digits of them, from the top, find the smallest one that stays and
 // how many equal to it do; then the entries that stay are numbered in order.  8 sequences of up to 8192 tokens, 8 heads:
-// 10.9 us, barriers and dependent steps on 64 of 256 compute units; one of 131071: four launches, 29 us in all.
+// 11.7 us, barriers and dependent steps on 64 of 256 compute units; one of 131071: four launches, 31.5 us in all.
 // paged_gather_kernel.  Entry r of those kept goes to position r on the pages of the new table.  Those are other pages
 // than the old ones, so no entry is read after it is overwritten and all are copied at once: 2048 entries of 8 sequences
-// (66 MB moved) 13.6 us, 4.8 TB/s, a large copy's rate being 4.9.
+// (66 MB moved) 13.5 us, 4.9 TB/s, a large copy's rate being 4.9.
 #include <hip/hip_runtime.h>
 
 #include "../../include/fa_gfx950.h"

@@ -64,7 +64,9 @@ def paged_attention(q, k_pages, v_pages, block_table, lens, window_size: Optiona
 
     max_seqlen: a bound on lens (default: the table's tokens); a tighter one makes the launch and its workspace
     smaller.  weight_sums (float32 [B, Hkv, tokens], at least max_seqlen tokens) accumulates the softmax weights in place:
-    weight_sums[b, h, k] += the sum of key k's weights over the query heads of KV head h, for paged_evict."""
+    weight_sums[b, h, k] += the sum of key k's weights over the query heads of KV head h, for paged_evict.  Its workspace is Hq / Hkv
+    times as large as weight_sums of max_seqlen tokens: a tight max_seqlen keeps it small.  Sinks in float32 save a
+    conversion on every call."""
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1])
     most = 2 ** 31 - 1

@@ -298,7 +298,9 @@ int fa_paged_append(const fa_paged_cache* c, const void* k, const void* v, const
  * that sees no key gets o = 0.  An infinite value that it sees makes o infinite (NaN with one of the other sign, and where its weight
  * underflows: 2^-32 of the largest for fp16, 2^-126 for the other types).  With weight_sums (float32 [batch, Hkv, at least min(max_len, table tokens)], NULL: none) the
  * softmax weights are accumulated: weight_sums[b, h, k] += sum over the query heads of KV head h of P[k], in a fixed
- * order.  max_len bounds lens (they are cut off there); it and the table's width size the grid and the workspace, of
+ * order; the workspace then holds a float32 score for each query head and key that a sequence of max_len tokens sees (at most
+ * window + sink of them), for every sequence: batch * heads_q * that many * 4 bytes, heads_q / heads_kv times the sums' own
+ * size, whatever lens are.  max_len bounds lens (they are cut off there); it and the table's width size the grid and the workspace, of
  * which at least fa_paged_workspace_bytes() are needed, 256-byte aligned. */
 typedef struct fa_paged_attention_params {
   fa_paged_cache cache;
