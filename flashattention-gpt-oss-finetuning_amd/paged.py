@@ -35,6 +35,7 @@ class _NoBackward(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, o, *inputs):
+        ctx.mark_dirty(o)  # (returned as it is and not as a view, so that it can be written in place)
         return o
 
     @staticmethod

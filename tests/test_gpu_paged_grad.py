@@ -29,3 +29,15 @@ def test_backward_raises(fa, gpu, monkeypatch, binding, which):
             o = run()
         assert not o.requires_grad
         same(o, want)
+
+
+def test_the_output_can_be_written(fa, gpu):
+    """A program that answers without no_grad, with the sinks as a parameter, and goes on in place."""
+    c = make(42, "bf16", "bf16", 64, 4, 2, 16, "hnd", (40, 9), nan=False)
+    t = {n: c[n].to(gpu) for n in ("q", "kp", "vp", "table", "lens", "sinks")}
+    run = lambda sinks: fa.paged_attention(t["q"], t["kp"], t["vp"], t["table"], t["lens"], sinks=sinks)
+    want = run(t["sinks"]) * 2 + 1
+    o = run(torch.nn.Parameter(t["sinks"]))
+    o.mul_(2)
+    o += 1
+    same(o.detach(), want)
